@@ -12,13 +12,11 @@
 //   bytes  8..11  the exporter's process id
 //   bytes 32..39  the allocation's size
 //   bytes 48..51  the exporter's process id again (HIP's part of the handle)
-// Nothing in it identifies the allocation beyond (pid, address): ROCr resolves
-// a handle when the peer OPENS it, by asking the exporter process -- its own
-// server thread on the abstract unix socket "hsa<pid>" -- for a DMA-buf of
-// whatever it holds at that address then (libhsa-runtime64.so.1.18.70200:
-// the "xhsa%i" / "%li" strings, connect + recvmsg on the attach side, accept +
-// strtoull + a map lookup + sendmsg(SCM_RIGHTS) in the server thread).  So a
-// handle is only as good as the exporter's address map at open time; libgeeps
+// Nothing in it identifies the allocation beyond (pid, address), and mappings
+// of correct handles were seen to hold another buffer that the exporter had
+// mapped (scripts/ipc_audit.py), as if what the exporter holds at that address
+// were looked up when the peer OPENS the handle.  So a handle is taken to be
+// only as good as the exporter's address map at open time; libgeeps
 // never frees an exported buffer while it runs (oplogs are retired, master
 // versions kept), never unmaps a mapping before Shutdown (an address that had
 // held a closed mapping was what the runtime misresolved: DESIGN.md §4), and

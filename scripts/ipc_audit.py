@@ -2,8 +2,8 @@
 tests/test_libgeeps.py writes them with GEEPS_TEST_LOG_DIR): for every mapping
 that failed its tag check, what the handle named, what the mapping held, and
 whether the EXPORTING process had itself mapped (imported) the buffer whose tag
-the mapping held -- the signature of the runtime's exporter handing out a
-DMA-buf of one of its imports instead of the buffer at the named address
+the mapping held -- the signature of the runtime's exporter handing out
+one of its imports instead of the buffer at the named address
 (DESIGN.md §4).
 
 `could_not_map` counts every failed device mapping (tag mismatches and the

@@ -6,15 +6,10 @@ and the 64-B handle as sixteen 32-bit words, so the fields the runtime puts
 in a handle (the exporter's pid? the buffer's address? a size? a counter?)
 can be read off by comparing words with known values.
 
-Why it matters: ROCr's non-legacy (DMA-buf) IPC, which this image runs
-(HSA_ENABLE_IPC_MODE_LEGACY=0), resolves a handle at OPEN time, not at export
-time -- libhsa-runtime64 runs a per-process server on the abstract unix socket
-"hsa<pid>" that takes a decimal id from the importer, looks it up in a map of
-exported ranges and exports a fresh DMA-buf for it, passed back by SCM_RIGHTS
-(objdump of libhsa-runtime64.so.1.18.70200: the "xhsa%i" / "%li" format
-strings, connect/recvmsg in the attach path, accept/strtoull/sendmsg in the
-server thread).  Whatever the handle names is therefore looked up in the
-exporter's state when the importer maps it.
+Why it matters: if the words hold nothing beyond the exporter's pid and the
+buffer's address and size, two buffers that held the same address at different
+times have the same handle, and only the exporter's state at the time the peer
+maps it can tell them apart.
 
 Usage: python scripts/probes/ipc_handle_layout.py   (one JSON line)
 """
