@@ -1,0 +1,642 @@
+// gp_route.hip — expert row routing (include/gp_reduce.h): the (token, choice)
+// pairs of a router grouped by expert, rows moved to their places there, the
+// places' rows brought back to the tokens with weights, and the gradient of
+// that.  The row gather / scatter-add of gp_kernels.hpp move rows through an
+// index that the host compiled; here the index is made on the device, in the
+// same step that uses it.
+//
+// The moves are bound by HBM: no row takes part in a product with another.
+
+#include "gp_device.hpp"
+
+namespace {
+
+constexpr int kSortBlock = 1024;
+constexpr int kSortWaves = kSortBlock / kWave;
+constexpr int kMaxExperts = 1024;  // one thread of a sort block each
+constexpr int kMaxChoices = kWave; // a token's choices lie in one wave's lanes
+
+// ---------------------------------------------------------------------------
+// Places: a stable counting sort of n = tokens * k choices by expert.
+//   counts[e]   = #{a : id[a] = e}
+//   offsets[e]  = sum over e' < e of counts[e'] rounded up to whole groups of `align`
+//   position[a] = offsets[id[a]] + #{b < a : id[b] = id[a]}
+// A block takes `per_block` choices in a row, a wave per_block / 16 of them, 64
+// at a step.  Within a step, lanes with the same id find each other by one
+// ballot per bit of the id; a lane's rank is the number of such lanes below
+// it, and the first of them moves the wave's own counter in LDS.  With one
+// block the counts of its waves are all there is; with more, route_count_kernel
+// has left every block's counts, and each block sums those before it.  Integer
+// sums only: the places do not depend on any order of arrival.
+// ---------------------------------------------------------------------------
+template <typename I>
+__device__ __forceinline__ int key_of(I id, int experts) {
+  return id >= 0 && id < (I)experts ? (int)id : experts;  // anything else: no expert here
+}
+
+template <typename I>
+__global__ __launch_bounds__(kSortBlock) void route_count_kernel(const I *__restrict__ ids, unsigned n,
+                                                                 unsigned per_block, int experts,
+                                                                 int *__restrict__ hist) {
+  __shared__ int count[kMaxExperts];
+  if ((int)threadIdx.x < experts) count[threadIdx.x] = 0;
+  __syncthreads();
+  const unsigned lo = blockIdx.x * per_block, hi = min(n, lo + per_block);
+  for (unsigned i = lo + threadIdx.x; i < hi; i += kSortBlock) {
+    const int key = key_of(ids[i], experts);
+    if (key < experts) atomicAdd(&count[key], 1);
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < experts) hist[(size_t)blockIdx.x * experts + threadIdx.x] = count[threadIdx.x];
+}
+
+struct SortShared {
+  int run[kSortWaves][kMaxExperts];  // a wave's next place in every expert's group
+  int total[kMaxExperts];
+  int before[kMaxExperts];  // choices of earlier blocks
+  int offset[kMaxExperts + 1];
+  int wave[kSortWaves];
+};
+
+// After it, s.run holds every wave's first places and s.total / s.offset the groups.
+template <typename I>
+__device__ void route_prepare(SortShared &s, const I *__restrict__ ids, unsigned lo, unsigned hi, unsigned per_wave,
+                              int experts, int align, const int *__restrict__ hist, unsigned block,
+                              unsigned blocks) {
+  const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
+  if (tid < experts) {
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) s.run[w][tid] = 0;
+    s.total[tid] = 0;
+    s.before[tid] = 0;
+  }
+  __syncthreads();
+  const unsigned from = min(hi, lo + wave * per_wave), to = min(hi, from + per_wave);
+  for (unsigned i = from + lane; i < to; i += kWave) {
+    const int key = key_of(ids[i], experts);
+    if (key < experts) atomicAdd(&s.run[wave][key], 1);
+  }
+  if (blocks > 1) {
+    const int parts = kSortBlock / experts;  // >= 1; thread (part, expert) sums every parts-th block's count
+    const int e = tid % experts, part = tid / experts;
+    if (part < parts) {
+      int total = 0, before = 0;
+#pragma unroll 8
+      for (unsigned g = part; g < blocks; g += parts) {
+        const int c = hist[(size_t)g * experts + e];
+        total += c;
+        before += g < block ? c : 0;
+      }
+      atomicAdd(&s.total[e], total);
+      atomicAdd(&s.before[e], before);
+    }
+  }
+  __syncthreads();
+  int mine = 0;
+  if (tid < experts) {
+    if (blocks == 1) {
+#pragma unroll
+      for (int w = 0; w < kSortWaves; ++w) mine += s.run[w][tid];
+      s.total[tid] = mine;
+    } else {
+      mine = s.total[tid];
+    }
+  }
+  int padded = (mine + align - 1) / align * align, scan = padded;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int up = __shfl_up(scan, d, kWave);
+    if (lane >= d) scan += up;
+  }
+  if (lane == kWave - 1) s.wave[wave] = scan;
+  __syncthreads();
+  int base = scan - padded;
+  for (int w = 0; w < wave; ++w) base += s.wave[w];
+  if (tid < experts) {
+    s.offset[tid] = base;
+    if (tid == experts - 1) s.offset[experts] = base + padded;
+    int at = base + s.before[tid];
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      const int c = s.run[w][tid];
+      s.run[w][tid] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+}
+
+// The wave's 64 choices of one step: each lane's place, or -1.
+__device__ __forceinline__ int route_step(SortShared &s, int key, int experts, int bits) {
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  uint64_t same = ~0ull;
+  for (int b = 0; b < bits; ++b) {
+    const uint64_t on = __ballot((key >> b) & 1);
+    same &= (key >> b) & 1 ? on : ~on;
+  }
+  const int rank = __popcll(same & ((1ull << lane) - 1));
+  const int first = __ffsll((long long)same) - 1;
+  int at = 0;
+  if (lane == first && key < experts) at = atomicAdd(&s.run[wave][key], __popcll(same));
+  at = __shfl(at, first, kWave) + rank;
+  return key < experts ? at : -1;
+}
+
+template <typename I>
+__global__ __launch_bounds__(kSortBlock) void route_place_kernel(
+    const I *__restrict__ ids, unsigned n, unsigned per_block, int experts, int bits, int align, unsigned rows,
+    const int *__restrict__ hist, int *__restrict__ position, int *__restrict__ order, int *__restrict__ counts,
+    int *__restrict__ offsets) {
+  __shared__ SortShared s;
+  const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
+  const unsigned lo = blockIdx.x * per_block, hi = min(n, lo + per_block);
+  const unsigned per_wave = per_block / kSortWaves;
+  route_prepare(s, ids, lo, hi, per_wave, experts, align, hist, blockIdx.x, gridDim.x);
+  if (blockIdx.x == 0) {
+    if (tid < experts) {
+      counts[tid] = s.total[tid];
+      offsets[tid] = s.offset[tid];
+    }
+    if (tid == 0) offsets[experts] = s.offset[experts];
+  }
+  const unsigned from = min(hi, lo + wave * per_wave), to = min(hi, from + per_wave);
+  for (unsigned i0 = from; i0 < to; i0 += kWave) {
+    const unsigned i = i0 + lane;
+    const int key = i < to ? key_of(ids[i], experts) : experts;
+    const int at = route_step(s, key, experts, bits);
+    if (i < to) position[i] = at;
+    if (at >= 0) order[at] = (int)i;
+  }
+  // places that hold no choice: the groups' padding, then all behind the last group
+  const unsigned waves = gridDim.x * kSortWaves, me = blockIdx.x * kSortWaves + wave;
+  for (unsigned e = me; e < (unsigned)experts; e += waves)
+    for (int p = s.offset[e] + s.total[e] + lane; p < s.offset[e + 1]; p += kWave) order[p] = -1;
+  for (unsigned p = s.offset[experts] + me * kWave + lane; p < rows; p += waves * kWave) order[p] = -1;
+}
+
+// ---------------------------------------------------------------------------
+// The moves.  A wave takes a token and a share of its columns, 64 lanes times
+// 16 bytes at a step, so x is read once however many choices a token has, and
+// every row of the grouped layout is touched once.
+// ---------------------------------------------------------------------------
+constexpr int kMoveBlock = 256;
+constexpr int kMoveWaves = kMoveBlock / kWave;
+constexpr unsigned kZeroRows = 16;  // places that one wave looks through for rows to clear
+
+struct Shape {
+  unsigned tokens, k, rows, width;
+  unsigned splits;       // waves that share a token's columns
+  unsigned token_waves;  // tokens * splits
+};
+
+// Rows that hold no choice are cleared, kZeroRows places to a wave.
+template <typename E>
+__device__ void clear_rows(E *__restrict__ out, size_t stride, const int *__restrict__ order, const Shape &d,
+                           unsigned wave) {
+  using V = Vec<E>;
+  const int lane = threadIdx.x % kWave;
+  const unsigned first = wave * kZeroRows;
+  const unsigned at = first + lane;
+  const bool mine = lane < (int)kZeroRows && at < d.rows;
+  const int o = mine ? order[at] : 0;
+  uint64_t empty = __ballot(mine && (o < 0 || (unsigned)o >= d.tokens * d.k));
+  while (empty) {
+    E *row = out + (size_t)(first + (__ffsll((long long)empty) - 1)) * stride;
+    empty &= empty - 1;
+    for (unsigned c = lane * V::N; c < d.width; c += kWave * V::N) {
+      const typename V::Raw zero = (E)0.0f;
+      if (c + V::N <= d.width)
+        store_raw(row + c, zero);
+      else
+        store_part(row + c, zero, d.width - c);
+    }
+  }
+}
+
+template <typename E>
+__global__ __launch_bounds__(kMoveBlock) void route_dispatch_kernel(E *__restrict__ out, size_t out_stride,
+                                                                    const E *__restrict__ x, size_t x_stride,
+                                                                    const int *__restrict__ position,
+                                                                    const int *__restrict__ order, Shape d) {
+  using V = Vec<E>;
+  const unsigned wave = blockIdx.x * kMoveWaves + threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave;
+  if (wave >= d.token_waves) {
+    clear_rows(out, out_stride, order, d, wave - d.token_waves);
+    return;
+  }
+  const unsigned t = wave / d.splits, split = wave % d.splits;
+  const int p = lane < (int)d.k ? position[(size_t)t * d.k + lane] : -1;
+  const uint64_t held = __ballot((unsigned)p < d.rows);
+  const E *from = x + (size_t)t * x_stride;
+  for (unsigned c = (split * kWave + lane) * V::N; c < d.width; c += d.splits * kWave * V::N) {
+    const bool whole = c + V::N <= d.width;
+    const typename V::Raw v = whole ? load_raw(from + c) : load_part(from + c, d.width - c);
+    for (uint64_t left = held; left; left &= left - 1) {
+      const int to = __builtin_amdgcn_readlane(p, __ffsll((long long)left) - 1);
+      E *row = out + (size_t)to * out_stride + c;
+      if (whole)
+        store_raw(row, v);
+      else
+        store_part(row, v, d.width - c);
+    }
+  }
+}
+
+// Weights: none (1), float, or the rows' own type.
+enum WeightType { kNoWeights = 0, kFloatWeights = 1, kRowWeights = 2 };
+
+template <typename E>
+__device__ __forceinline__ float weight_at(const void *w, int type, size_t i) {
+  return type == kFloatWeights ? static_cast<const float *>(w)[i]
+         : type == kRowWeights ? (float)static_cast<const E *>(w)[i]
+                               : 1.0f;
+}
+
+// G held choices from `left` on: their rows' 16 bytes are all asked for before
+// the first is used.
+template <typename E, int G>
+__device__ __forceinline__ void combine_group(typename Vec<E>::F &acc, uint64_t &left, const E *__restrict__ rows,
+                                              size_t stride, int p, float w, unsigned c, bool whole, unsigned width) {
+  using V = Vec<E>;
+  typename V::Raw v[G];
+  float f[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const int from = __ffsll((long long)left) - 1;
+    left &= left - 1;
+    const E *row = rows + (size_t)__builtin_amdgcn_readlane(p, from) * stride + c;
+    f[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), from));
+    v[g] = whole ? load_raw(row) : load_part(row, width - c);
+  }
+#pragma unroll
+  for (int g = 0; g < G; ++g) acc += f[g] * to_float<E>(v[g]);  // choices in order, in 32 bits
+}
+
+template <typename E>
+__global__ __launch_bounds__(kMoveBlock) void route_combine_kernel(E *__restrict__ y, size_t y_stride,
+                                                                   const E *__restrict__ rows, size_t row_stride,
+                                                                   const int *__restrict__ position,
+                                                                   const void *__restrict__ weights, int weight_type,
+                                                                   Shape d) {
+  using V = Vec<E>;
+  const unsigned wave = blockIdx.x * kMoveWaves + threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave;
+  if (wave >= d.token_waves) return;
+  const unsigned t = wave / d.splits, split = wave % d.splits;
+  const size_t a = (size_t)t * d.k + lane;
+  const int p = lane < (int)d.k ? position[a] : -1;
+  const float w = lane < (int)d.k ? weight_at<E>(weights, weight_type, a) : 0.0f;
+  const uint64_t held = __ballot((unsigned)p < d.rows);
+  E *to = y + (size_t)t * y_stride;
+  for (unsigned c = (split * kWave + lane) * V::N; c < d.width; c += d.splits * kWave * V::N) {
+    const bool whole = c + V::N <= d.width;
+    typename V::F acc = 0.0f;
+    uint64_t left = held;
+    int n = __popcll(held);
+    for (; n >= 8; n -= 8) combine_group<E, 8>(acc, left, rows, row_stride, p, w, c, whole, d.width);
+    if (n >= 4) combine_group<E, 4>(acc, left, rows, row_stride, p, w, c, whole, d.width), n -= 4;
+    if (n >= 2) combine_group<E, 2>(acc, left, rows, row_stride, p, w, c, whole, d.width), n -= 2;
+    if (n >= 1) combine_group<E, 1>(acc, left, rows, row_stride, p, w, c, whole, d.width);
+    if (whole)
+      store_raw(to + c, from_float<E>(acc));
+    else
+      store_part(to + c, from_float<E>(acc), d.width - c);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The gradient of combine: d_rows[position[a]] = w[a] * dy[t], d_w[a] = dy[t] .
+// rows[position[a]].  dy is read once per group of up to 8 choices; the dots
+// are 32-bit sums, lane by lane, then over the wave, then over the splits' waves
+// in their order.
+// ---------------------------------------------------------------------------
+template <typename E, int G>
+__device__ __forceinline__ void grad_group(uint64_t &left, E *__restrict__ d_rows, size_t d_stride,
+                                           const E *__restrict__ dy, const E *__restrict__ rows, size_t row_stride,
+                                           int p, float w, unsigned first, unsigned step, unsigned width, float &dot) {
+  using V = Vec<E>;
+  const int lane = threadIdx.x % kWave;
+  int from[G];
+  float f[G], sum[G];
+  size_t at[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    from[g] = __ffsll((long long)left) - 1;
+    left &= left - 1;
+    at[g] = (size_t)__builtin_amdgcn_readlane(p, from[g]);
+    f[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), from[g]));
+    sum[g] = 0.0f;
+  }
+  for (unsigned c = first; c < width; c += step) {
+    const bool whole = c + V::N <= width;
+    const int part = (int)(width - c);
+    const typename V::F o = to_float<E>(whole ? load_raw(dy + c) : load_part(dy + c, part));
+    typename V::Raw v[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const E *row = rows + at[g] * row_stride + c;
+      v[g] = whole ? load_raw(row) : load_part(row, part);
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const typename V::F r = to_float<E>(v[g]);
+#pragma unroll
+      for (int i = 0; i < V::N; ++i) sum[g] += o[i] * r[i];
+      E *row = d_rows + at[g] * d_stride + c;
+      const typename V::Raw out = from_float<E>(f[g] * o);
+      if (whole)
+        store_raw(row, out);
+      else
+        store_part(row, out, part);
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    const float total = wave_sum(sum[g]);
+    if (lane == from[g]) dot = total;
+  }
+}
+
+// S waves share a token (d.splits = S); a block holds kMoveWaves / S tokens.
+template <typename E, int S>
+__global__ __launch_bounds__(kMoveBlock) void route_combine_grad_kernel(
+    E *__restrict__ d_rows, size_t d_stride, void *__restrict__ d_weights, const E *__restrict__ dy, size_t dy_stride,
+    const E *__restrict__ rows, size_t row_stride, const int *__restrict__ position, const int *__restrict__ order,
+    const void *__restrict__ weights, int weight_type, Shape d) {
+  using V = Vec<E>;
+  __shared__ float part[kMoveWaves][kWave];
+  const unsigned in_block = threadIdx.x / kWave;
+  const unsigned wave = blockIdx.x * kMoveWaves + in_block;
+  const int lane = threadIdx.x % kWave;
+  const bool moves = wave < d.token_waves;
+  if (!moves) {  // these waves clear, and meet the others at the barrier below
+    clear_rows(d_rows, d_stride, order, d, wave - d.token_waves);
+  }
+  const unsigned t = wave / S, split = wave % S;
+  const size_t a = (size_t)t * d.k + lane;
+  const bool mine = moves && lane < (int)d.k;
+  const int p = mine ? position[a] : -1;
+  const uint64_t held = __ballot((unsigned)p < d.rows);
+  float dot = 0.0f;
+  if (moves) {
+    const float w = mine ? weight_at<E>(weights, weight_type, a) : 0.0f;
+    const E *o = dy + (size_t)t * dy_stride;
+    const unsigned first = (split * kWave + lane) * V::N, step = S * kWave * V::N;
+    uint64_t left = held;
+    int n = __popcll(held);
+    for (; n >= 8; n -= 8) grad_group<E, 8>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot);
+    if (n >= 4) grad_group<E, 4>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot), n -= 4;
+    if (n >= 2) grad_group<E, 2>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot), n -= 2;
+    if (n >= 1) grad_group<E, 1>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot);
+  }
+  if constexpr (S > 1) {
+    part[in_block][lane] = dot;
+    __syncthreads();
+    if (split == 0) {
+      dot = 0.0f;
+#pragma unroll
+      for (int s = 0; s < S; ++s) dot += part[in_block + s][lane];
+    }
+  }
+  if (mine && split == 0) {
+    if (weight_type == kRowWeights)
+      static_cast<E *>(d_weights)[a] = (E)dot;
+    else
+      static_cast<float *>(d_weights)[a] = dot;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------
+constexpr size_t kSingleSort = 8192;   // choices that one block places
+constexpr size_t kMostSortBlocks = 256;
+
+struct SortPlan {
+  unsigned blocks, per_block;
+  int bits;
+};
+
+SortPlan sort_plan(size_t n, size_t experts) {
+  SortPlan p;
+  const size_t unit = kSortBlock;  // every wave takes whole steps of 64
+  size_t per = n <= kSingleSort ? n : 4 * unit;
+  if (n > kSingleSort && (n + per - 1) / per > kMostSortBlocks) per = (n + kMostSortBlocks - 1) / kMostSortBlocks;
+  per = per ? (per + unit - 1) / unit * unit : unit;
+  p.per_block = (unsigned)per;
+  p.blocks = (unsigned)((n + per - 1) / per);
+  p.bits = 1;
+  while ((1u << p.bits) < experts + 1) ++p.bits;  // `experts` itself stands for no expert
+  return p;
+}
+
+int check_groups(size_t tokens, size_t k, size_t experts, size_t align) {
+  GP_REQUIRE(k >= 1 && k <= (size_t)kMaxChoices, "choices per token must be 1 to 64");
+  GP_REQUIRE(experts >= 1 && experts <= (size_t)kMaxExperts, "experts must be 1 to 1024");
+  GP_REQUIRE(align >= 1 && align <= (1u << 20), "align must be 1 to 2^20");
+  GP_REQUIRE(tokens <= (size_t)INT32_MAX / k, "tokens * choices must be under 2^31");
+  const size_t n = tokens * k;
+  GP_REQUIRE(n + (n < experts ? n : experts) * (align - 1) <= (size_t)INT32_MAX, "grouped rows must be under 2^31");
+  return GP_OK;
+}
+
+size_t grouped_rows(size_t tokens, size_t k, size_t experts, size_t align) {
+  const size_t n = tokens * k;
+  return (n + (n < experts ? n : experts) * (align - 1)) / align * align;
+}
+
+int check_move(size_t tokens, size_t k, size_t rows, size_t width, int type) {
+  GP_REQUIRE(type_known(type), "row type must be GP_F32, GP_BF16 or GP_F16");
+  GP_REQUIRE(k >= 1 && k <= (size_t)kMaxChoices, "choices per token must be 1 to 64");
+  GP_REQUIRE(tokens <= (size_t)INT32_MAX / k, "tokens * choices must be under 2^31");
+  GP_REQUIRE(rows <= (size_t)INT32_MAX, "grouped rows must be under 2^31");
+  GP_REQUIRE(width <= (1u << 24), "row width must be at most 2^24");
+  return GP_OK;
+}
+
+// Waves over a token's columns: enough of them to fill the chip when tokens
+// are few, one when tokens alone do.
+unsigned pick_splits(size_t tokens, size_t width, int type) {
+  const size_t per_step = kWave * 16 / type_size(type);
+  const size_t steps = (width + per_step - 1) / per_step;
+  const size_t want = (size_t)device_cus() * 16;  // 4 waves per SIMD
+  size_t s = tokens ? want / tokens : 1;
+  if (s < 1) s = 1;
+  return (unsigned)(s < steps ? s : (steps ? steps : 1));
+}
+
+int check_grid(size_t waves, unsigned *blocks) {
+  const size_t b = (waves + kMoveWaves - 1) / kMoveWaves;
+  GP_REQUIRE(b <= (size_t)INT32_MAX, "too many rows for one launch");
+  *blocks = (unsigned)b;
+  return GP_OK;
+}
+
+#define GP_TRY(expr)             \
+  do {                           \
+    const int rc_ = (expr);      \
+    if (rc_ != GP_OK) return rc_; \
+  } while (0)
+
+// f(E{}) with the element type of `type`.
+template <typename F>
+void with_type(int type, F f) {
+  if (type == GP_F32)
+    f((float)0);
+  else if (type == GP_BF16)
+    f((__bf16)0.0f);
+  else
+    f((_Float16)0);
+}
+
+template <typename I>
+void launch_sort(const void *ids, const SortPlan &p, size_t n, int experts, int align, size_t rows, int *position,
+                 int *order, int *counts, int *offsets, int *hist, hipStream_t s) {
+  const I *in = static_cast<const I *>(ids);
+  if (p.blocks > 1)
+    hipLaunchKernelGGL((route_count_kernel<I>), dim3(p.blocks), dim3(kSortBlock), 0, s, in, (unsigned)n, p.per_block,
+                       experts, hist);
+  hipLaunchKernelGGL((route_place_kernel<I>), dim3(p.blocks), dim3(kSortBlock), 0, s, in, (unsigned)n, p.per_block,
+                     experts, p.bits, align, (unsigned)rows, (const int *)hist, position, order, counts, offsets);
+}
+
+size_t strided_bytes(size_t rows, size_t stride, size_t width, int type) {
+  return rows && width ? ((rows - 1) * stride + width) * type_size(type) : 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gp_route_rows(size_t tokens, size_t k, size_t experts, size_t align, size_t *rows) {
+  GP_REQUIRE(rows, "null rows");
+  GP_TRY(check_groups(tokens, k, experts, align));
+  *rows = grouped_rows(tokens, k, experts, align);
+  return GP_OK;
+}
+
+int gp_route_workspace(size_t tokens, size_t k, size_t experts, size_t *bytes) {
+  GP_REQUIRE(bytes, "null bytes");
+  GP_TRY(check_groups(tokens, k, experts, 1));
+  const SortPlan p = sort_plan(tokens * k, experts);
+  *bytes = p.blocks > 1 ? (size_t)p.blocks * experts * sizeof(int) : 0;
+  return GP_OK;
+}
+
+int gp_route_sort(const void *ids, int id_bits, size_t tokens, size_t k, size_t experts, size_t align,
+                  int32_t *position, int32_t *order, int32_t *counts, int32_t *offsets, void *workspace,
+                  size_t workspace_bytes, gp_stream s) {
+  GP_REQUIRE(id_bits == 32 || id_bits == 64, "ids must be 32 or 64 bits wide");
+  size_t need = 0;
+  GP_TRY(check_groups(tokens, k, experts, align));
+  GP_TRY(gp_route_workspace(tokens, k, experts, &need));
+  GP_REQUIRE(counts && offsets, "null counts or offsets");
+  const size_t n = tokens * k;
+  GP_REQUIRE(n == 0 || (ids && position && order), "null ids, position or order");
+  GP_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "workspace missing or too small");
+  SortPlan p = sort_plan(n, experts);
+  if (p.blocks == 0) p.blocks = 1;  // no tokens: the empty groups
+  const size_t rows = grouped_rows(tokens, k, experts, align);
+  int *hist = static_cast<int *>(workspace);
+  if (id_bits == 64)
+    launch_sort<int64_t>(ids, p, n, (int)experts, (int)align, rows, position, order, counts, offsets, hist,
+                         (hipStream_t)s);
+  else
+    launch_sort<int32_t>(ids, p, n, (int)experts, (int)align, rows, position, order, counts, offsets, hist,
+                         (hipStream_t)s);
+  GP_HIP_TRY(hipGetLastError());
+  return GP_OK;
+}
+
+int gp_route_dispatch(void *out, size_t out_stride, const void *x, size_t x_stride, int type,
+                      const int32_t *position, const int32_t *order, size_t tokens, size_t k, size_t rows,
+                      size_t width, gp_stream s) {
+  GP_TRY(check_move(tokens, k, rows, width, type));
+  if (rows == 0 || width == 0) return GP_OK;
+  GP_REQUIRE(out && order && (tokens == 0 || (x && position)), "null out, x, position or order");
+  GP_REQUIRE(out_stride >= width && x_stride >= width, "row stride smaller than the width");
+  GP_REQUIRE(!bytes_overlap(out, strided_bytes(rows, out_stride, width, type), x,
+                            strided_bytes(tokens, x_stride, width, type)),
+             "out overlaps x");
+  Shape d{(unsigned)tokens, (unsigned)k, (unsigned)rows, (unsigned)width, pick_splits(tokens, width, type), 0};
+  const size_t waves = tokens * (size_t)d.splits;
+  unsigned blocks = 0;
+  GP_TRY(check_grid(waves + (rows + kZeroRows - 1) / kZeroRows, &blocks));
+  d.token_waves = (unsigned)waves;
+  with_type(type, [&](auto e) {
+    using E = decltype(e);
+    hipLaunchKernelGGL((route_dispatch_kernel<E>), dim3(blocks), dim3(kMoveBlock), 0, (hipStream_t)s,
+                       static_cast<E *>(out), out_stride, static_cast<const E *>(x), x_stride, position, order, d);
+  });
+  GP_HIP_TRY(hipGetLastError());
+  return GP_OK;
+}
+
+int gp_route_combine(void *y, size_t y_stride, const void *rows_in, size_t row_stride, int type,
+                     const int32_t *position, const void *weights, int weight_type, size_t tokens, size_t k,
+                     size_t rows, size_t width, gp_stream s) {
+  GP_TRY(check_move(tokens, k, rows, width, type));
+  GP_REQUIRE(!weights || weight_type == GP_F32 || weight_type == type, "weights must be GP_F32 or of the rows' type");
+  if (tokens == 0 || width == 0) return GP_OK;
+  GP_REQUIRE(y && position && (rows == 0 || rows_in), "null y, rows or position");
+  GP_REQUIRE(y_stride >= width && row_stride >= width, "row stride smaller than the width");
+  GP_REQUIRE(!bytes_overlap(y, strided_bytes(tokens, y_stride, width, type), rows_in,
+                            strided_bytes(rows, row_stride, width, type)),
+             "y overlaps the rows");
+  const int wt = !weights ? kNoWeights : weight_type == GP_F32 ? kFloatWeights : kRowWeights;
+  Shape d{(unsigned)tokens, (unsigned)k, (unsigned)rows, (unsigned)width, pick_splits(tokens, width, type), 0};
+  const size_t waves = tokens * (size_t)d.splits;
+  unsigned blocks = 0;
+  GP_TRY(check_grid(waves, &blocks));
+  d.token_waves = (unsigned)waves;
+  with_type(type, [&](auto e) {
+    using E = decltype(e);
+    hipLaunchKernelGGL((route_combine_kernel<E>), dim3(blocks), dim3(kMoveBlock), 0, (hipStream_t)s,
+                       static_cast<E *>(y), y_stride, static_cast<const E *>(rows_in), row_stride, position, weights,
+                       wt, d);
+  });
+  GP_HIP_TRY(hipGetLastError());
+  return GP_OK;
+}
+
+int gp_route_combine_grad(void *d_rows, size_t d_stride, void *d_weights, const void *dy, size_t dy_stride,
+                          const void *rows_in, size_t row_stride, int type, const int32_t *position,
+                          const int32_t *order, const void *weights, int weight_type, size_t tokens, size_t k,
+                          size_t rows, size_t width, gp_stream s) {
+  GP_TRY(check_move(tokens, k, rows, width, type));
+  GP_REQUIRE(weight_type == GP_F32 || weight_type == type, "weights must be GP_F32 or of the rows' type");
+  if (tokens == 0 && rows == 0) return GP_OK;
+  GP_REQUIRE(tokens == 0 || (position && weights && d_weights), "null position or weights");
+  GP_REQUIRE(rows == 0 || order, "null order");
+  GP_REQUIRE(width == 0 || ((tokens == 0 || dy) && (rows == 0 || (d_rows && rows_in))), "null dy, rows or d_rows");
+  GP_REQUIRE(d_stride >= width && dy_stride >= width && row_stride >= width, "row stride smaller than the width");
+  const size_t db = strided_bytes(rows, d_stride, width, type), rb = strided_bytes(rows, row_stride, width, type);
+  const size_t yb = strided_bytes(tokens, dy_stride, width, type);
+  // in place (the same rows and stride) every element is read before it is written, by the same lane
+  GP_REQUIRE(!bytes_overlap(d_rows, db, dy, yb), "d_rows overlaps dy");
+  GP_REQUIRE(!bytes_overlap(d_rows, db, rows_in, rb), "d_rows overlaps the rows");
+  const int wt = weight_type == GP_F32 ? kFloatWeights : kRowWeights;
+  const unsigned splits = pick_splits(tokens, width, type) > 1 ? 4 : 1;
+  Shape d{(unsigned)tokens, (unsigned)k, (unsigned)rows, (unsigned)width, splits, 0};
+  const size_t waves = tokens * (size_t)d.splits;
+  unsigned blocks = 0;
+  GP_TRY(check_grid(waves + (rows + kZeroRows - 1) / kZeroRows, &blocks));
+  d.token_waves = (unsigned)waves;
+  with_type(type, [&](auto e) {
+    using E = decltype(e);
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kMoveBlock), 0, (hipStream_t)s, static_cast<E *>(d_rows), d_stride,
+                         d_weights, static_cast<const E *>(dy), dy_stride, static_cast<const E *>(rows_in), row_stride,
+                         position, order, weights, wt, d);
+    };
+    if (splits == 4)
+      go(route_combine_grad_kernel<E, 4>);
+    else
+      go(route_combine_grad_kernel<E, 1>);
+  });
+  GP_HIP_TRY(hipGetLastError());
+  return GP_OK;
+}
+
+}  // extern "C"

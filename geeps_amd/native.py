@@ -34,6 +34,9 @@ class DoubleIndex(ctypes.Structure):
 
 
 GP_MAX_SEGMENTS = 64  # include/gp_reduce.h
+GP_F32, GP_BF16, GP_F16 = 0, 1, 2
+GP_CLIP_WORKSPACE_BYTES = 16384
+GP_CLIP_PROPAGATE, GP_CLIP_SKIP = 0, 1
 
 
 class RowSegments(ctypes.Structure):
@@ -105,6 +108,21 @@ _SIGNATURES = {
     "gp_host_add": (_i, [_sz, _vp, _vp]),
     "gp_host_zero": (_i, [_sz, _vp]),
     "gp_zero": (_i, [_vp, _sz, _vp]),
+    "gp_route_rows": (_i, [_sz, _sz, _sz, _sz, _c.POINTER(_sz)]),
+    "gp_route_workspace": (_i, [_sz, _sz, _sz, _c.POINTER(_sz)]),
+    "gp_route_sort": (_i, [_vp, _i, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "gp_route_dispatch": (_i, [_vp, _sz, _vp, _sz, _i, _vp, _vp, _sz, _sz, _sz, _sz, _vp]),
+    "gp_route_combine": (_i, [_vp, _sz, _vp, _sz, _i, _vp, _vp, _i, _sz, _sz, _sz, _sz, _vp]),
+    "gp_route_combine_grad": (_i, [_vp, _sz, _vp, _vp, _sz, _vp, _sz, _i, _vp, _vp, _vp, _i, _sz, _sz, _sz,
+                                   _sz, _vp]),
+    "gp_grad_plan_create": (_i, [_c.POINTER(_vp), _sz, _c.POINTER(_vp), _c.POINTER(_i), _c.POINTER(_vp),
+                                 _c.POINTER(_i), _c.POINTER(_sz)]),
+    "gp_grad_plan_destroy": (_i, [_vp]),
+    "gp_grad_sum_squares": (_i, [_vp, _vp, _vp, _vp]),
+    "gp_grad_clip": (_i, [_vp, _c.c_double, _c.c_double, _i, _vp, _vp, _vp, _vp]),
+    "gp_bucket_sum_clipped": (_i, [_vp, _vp, _c.POINTER(_vp), _i, _sz, _vp, _c.c_double, _c.c_double, _i, _vp,
+                                   _vp, _vp, _vp]),
+    "gp_bucket_sum_squares": (_i, [_vp, _c.POINTER(_vp), _i, _sz, _vp, _vp, _vp]),
     "gp_hbm_probe": (_i, [_i, _vp, _sz, _vp]),
     "gp_device_count": (_i, [_c.POINTER(_i)]),
     "gp_set_device": (_i, [_i]),

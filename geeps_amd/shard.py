@@ -24,7 +24,11 @@ Here the same three steps run over RCCL (``torch.distributed`` backend "nccl"
 Clients are synthetic and hosted round-robin: client ``c`` lives on rank
 ``c % world``; every rank hosts ``num_clients // world`` of them.
 
-``apply_fn`` exists so the gloo/CPU tests can exercise the exchange and
+With ``max_norm`` the clock's update is bounded: the shards' sums of squares are
+added up over the ranks (one all-reduced float64 value) and every shard adds the
+sum of its buckets scaled to that norm (clipping.apply_updates_clipped).
+
+``apply_fn`` (and ``clip_fns`` for a bounded update) exists so the gloo/CPU tests can exercise the exchange and
 partition logic with the oracle standing in for the HIP kernel; the product
 default is the HIP kernel and nothing here falls back to the CPU.
 """
@@ -58,6 +62,16 @@ def _default_apply(master: torch.Tensor, buckets: Sequence[torch.Tensor]) -> Non
     bucket_sum_apply(master, buckets)
 
 
+def _default_squares(updates: Sequence[torch.Tensor], scratch) -> torch.Tensor:
+    from .clipping import sum_updates_squares
+    return sum_updates_squares(updates, scratch)
+
+
+def _default_clipped(master, updates, max_norm, scratch, total) -> torch.Tensor:
+    from .clipping import apply_updates_clipped
+    return apply_updates_clipped(master, updates, max_norm, scratch=scratch, total=total)
+
+
 @dataclass
 class ShardLayout:
     num_rows: int
@@ -87,13 +101,16 @@ class ShardedReducer:
 
     ``deltas[j]`` is the full-table delta buffer (num_rows * row_size floats) of
     hosted client ``hosted[j]``.  ``push()`` runs the exchange, ``apply()`` the
-    device-resident N-way sum, ``refresh()`` the all-gather.
+    device-resident N-way sum, ``refresh()`` the all-gather.  With ``max_norm``
+    ``apply()`` bounds the norm of the whole table's summed update, over all
+    shards, and leaves it in ``norm`` (a device value, the same on every rank).
     """
 
     def __init__(self, num_rows: int, row_size: int, num_clients: int, device,
                  group=None, exchange: str = "a2a",
                  apply_fn: Callable | None = None, master: torch.Tensor | None = None,
-                 layout: str = "arena"):
+                 layout: str = "arena", max_norm: float | None = None,
+                 clip_fns: tuple[Callable, Callable] | None = None):
         if exchange not in ("a2a", "rs"):
             raise ValueError("exchange must be 'a2a' or 'rs'")
         self.group = group
@@ -105,6 +122,12 @@ class ShardedReducer:
         self.exchange = exchange
         self.device = device
         self.apply_fn = apply_fn or _default_apply
+        if max_norm is not None and not max_norm >= 0.0:
+            raise ValueError("max_norm must not be negative or NaN")
+        self.max_norm = max_norm
+        self.squares_fn, self.clipped_fn = clip_fns or (_default_squares, _default_clipped)
+        self.norm = None
+        self._scratch = None
         if layout not in ("arena", "separate"):
             raise ValueError("layout must be 'arena' or 'separate'")
         L = self.layout
@@ -187,7 +210,17 @@ class ShardedReducer:
             buckets = self._buckets
         else:
             buckets = [b[:L.local_vals] for b in self._buckets]
-        self.apply_fn(self.master[:L.local_vals], buckets)
+        master = self.master[:L.local_vals]
+        if self.max_norm is None:
+            self.apply_fn(master, buckets)
+            return
+        if self._scratch is None and len(buckets) > 2:  # holds the sum between its two passes
+            self._scratch = torch.empty(L.local_vals, dtype=torch.float32, device=self.device)
+        total = None
+        if self.world > 1:
+            total = self.squares_fn(buckets, self._scratch)
+            dist.all_reduce(total, group=self.group)
+        self.norm = self.clipped_fn(master, buckets, self.max_norm, self._scratch, total)
 
     # -- refresh ------------------------------------------------------------
     def refresh(self) -> torch.Tensor:

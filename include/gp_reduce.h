@@ -360,6 +360,105 @@ int gp_bucket_sum_launch_plan(size_t num_vals, int num_buckets, gp_sum_plan *pla
  * src/common/row-op-util.hpp:72-79) as gp_add(n, y, x, y). In-place allowed. */
 int gp_add(size_t n, const float *a, const float *b, float *y, gp_stream s);
 
+/* ---------------------------------------------------------------------------
+ * Expert row routing: the row moves of a layer of experts, whose index is made
+ * on the device from a router's choices in the same step.  Rows are `width`
+ * values of one type at base + r * stride (strides in values, at least the
+ * width); 32-bit sums whatever the type.  No reference counterpart.
+ *
+ * ids[t * k + c] is the expert of token t's choice c; anything outside
+ * [0, experts) means no expert here (padding, an expert of another rank): the
+ * choice has no row.  The grouped layout holds every expert's rows together,
+ * tokens in order, each group rounded up to a multiple of `align` rows, in a
+ * fixed gp_route_rows() rows so that no size comes back from the device:
+ *   counts[e]   = choices of expert e
+ *   offsets[e]  = first row of e's group; offsets[experts] = end of the last
+ *   position[a] = row of choice a = t * k + c, or -1
+ *   order[r]    = choice in row r, or -1 (a group's padding, behind the last)
+ * k 1..64, experts 1..1024, tokens * k and the rows under 2^31.
+ * ------------------------------------------------------------------------- */
+#define GP_F32 0
+#define GP_BF16 1
+#define GP_F16 2
+
+/* Rows of the grouped layout: tokens * k and align - 1 for every expert that
+ * can have a row, rounded down to whole groups. */
+int gp_route_rows(size_t tokens, size_t k, size_t experts, size_t align, size_t *rows);
+/* Device scratch of one gp_route_sort (0 for a short one, which may pass NULL). */
+int gp_route_workspace(size_t tokens, size_t k, size_t experts, size_t *bytes);
+/* The layout of `ids` (device, id_bits 32 or 64, signed).  position: tokens * k,
+ * order: gp_route_rows(), counts: experts, offsets: experts + 1 entries. */
+int gp_route_sort(const void *ids, int id_bits, size_t tokens, size_t k, size_t experts, size_t align,
+                  int32_t *position, int32_t *order, int32_t *counts, int32_t *offsets, void *workspace,
+                  size_t workspace_bytes, gp_stream s);
+/* out[r] = x[order[r] / k], zeros where order[r] < 0, for every r < rows; out
+ * must not overlap x. */
+int gp_route_dispatch(void *out, size_t out_stride, const void *x, size_t x_stride, int type,
+                      const int32_t *position, const int32_t *order, size_t tokens, size_t k, size_t rows,
+                      size_t width, gp_stream s);
+/* y[t] = sum over c of weights[t * k + c] * rows_in[position[t * k + c]],
+ * choices in order, those without a row left out (a token with none: zeros).
+ * weights: GP_F32 or the rows' type; NULL: 1 each, which is the gradient of
+ * gp_route_dispatch.  y must not overlap the rows. */
+int gp_route_combine(void *y, size_t y_stride, const void *rows_in, size_t row_stride, int type,
+                     const int32_t *position, const void *weights, int weight_type, size_t tokens, size_t k,
+                     size_t rows, size_t width, gp_stream s);
+/* The gradient of gp_route_combine with weights, for dy = its y's:
+ *   d_rows[r] = weights[order[r]] * dy[order[r] / k], zeros where order[r] < 0
+ *   d_weights[a] = dy[a / k] . rows_in[position[a]], 0 where position[a] < 0
+ * d_weights has the weights' type; d_rows must not overlap dy or the rows. */
+int gp_route_combine_grad(void *d_rows, size_t d_stride, void *d_weights, const void *dy, size_t dy_stride,
+                          const void *rows_in, size_t row_stride, int type, const int32_t *position,
+                          const int32_t *order, const void *weights, int weight_type, size_t tokens, size_t k,
+                          size_t rows, size_t width, gp_stream s);
+
+/* ---------------------------------------------------------------------------
+ * Updates scaled to a bound on their norm.  No reference counterpart.
+ *   norm = sqrt(sum of squares over everything listed), in 64 bits
+ *   f    = scale * (norm <= max_norm ? 1 : max_norm / norm), rounded to 32 bits
+ * max_norm >= 0 (infinity: no bound), scale finite.  A norm that is infinite or
+ * NaN makes f 0 or NaN and the outputs NaN where the values are no numbers
+ * (GP_CLIP_PROPAGATE), or drops the update: zeros, an unchanged master
+ * (GP_CLIP_SKIP).  `workspace`: GP_CLIP_WORKSPACE_BYTES of device memory, 8-B
+ * aligned, any contents, one for each call in flight.  `norm` (device, may be
+ * NULL) gets the norm.  Same inputs, same bits.
+ * With `sum` (device) given, its sum of squares is used and the values are not
+ * squared again: the way to a norm over several lists, tables or ranks, whose
+ * gp_*_sum_squares are added up in between.
+ * ------------------------------------------------------------------------- */
+#define GP_CLIP_WORKSPACE_BYTES 16384
+#define GP_CLIP_PROPAGATE 0
+#define GP_CLIP_SKIP 1
+
+/* A list of gradients and the buffers that their scaled values go to, compiled
+ * once.  grads[i], outs[i]: device, sizes[i] values (0: skipped); outs[i] may be
+ * grads[i] (in place), has its type or GP_F32, and overlaps nothing else.  The
+ * plan's table lives on the current device, and the plan runs only there; it
+ * holds the pointers, not the memory.  Creating one allocates and copies, so not
+ * while a stream is being captured. */
+typedef struct gp_grad_plan_s *gp_grad_plan;
+int gp_grad_plan_create(gp_grad_plan *plan, size_t count, const void *const *grads, const int *grad_types,
+                        void *const *outs, const int *out_types, const size_t *sizes);
+int gp_grad_plan_destroy(gp_grad_plan plan);
+/* *sum (device) = the sum of squares of the plan's gradients. */
+int gp_grad_sum_squares(gp_grad_plan plan, double *sum, void *workspace, gp_stream s);
+/* outs[i] = f * grads[i], one rounding to the output's type. */
+int gp_grad_clip(gp_grad_plan plan, double max_norm, double scale, int nonfinite, const double *sum, float *norm,
+                 void *workspace, gp_stream s);
+/* The server's sum of N client deltas (gp_bucket_sum_apply's `buckets`), as an
+ * update of bounded norm: u = ((b[0] + b[1]) + ...) + b[N-1] in 32 bits, and
+ *   out[i] = in[i] + f * u[i]
+ * with the norm of u.  out may be in; it overlaps no bucket.  `scratch`:
+ * num_vals floats that hold u between the passes, overlapping none of the
+ * others; unused (may be NULL) below three buckets. */
+int gp_bucket_sum_clipped(float *out, const float *in, const float *const *buckets, int num_buckets,
+                          size_t num_vals, float *scratch, double max_norm, double scale, int nonfinite,
+                          const double *sum, float *norm, void *workspace, gp_stream s);
+/* *sum (device) = the sum of squares of u; from three buckets on, `scratch` = u,
+ * which gp_bucket_sum_clipped with `sum` given takes from there. */
+int gp_bucket_sum_squares(float *scratch, const float *const *buckets, int num_buckets, size_t num_vals,
+                          double *sum, void *workspace, gp_stream s);
+
 /* HBM probe for measurement tools: stream `num_vals` floats of a 16-B
  * aligned device buffer once, read-only (GP_PROBE_READ: 16-B non-temporal
  * loads; the buffer is not written) or write-only (GP_PROBE_WRITE: zeros,
