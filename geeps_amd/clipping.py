@@ -23,7 +23,7 @@ import torch
 
 from . import native
 from .native import check
-from .routing import _On, _TYPES
+from .routing import _On, _TYPES, _current_device, _current_stream
 
 
 def _bound(max_norm, scale, skip_nonfinite):
@@ -104,10 +104,12 @@ class GradPlan:
     def sum_squares(self, stream=None) -> torch.Tensor:
         """The sum of the gradients' squares: one float64 value."""
         self._open()
-        with _On(self.device, stream) as ptr:
-            total = torch.empty((), dtype=torch.float64, device=self.device)
-            check(native.lib().gp_grad_sum_squares(self._h, total.data_ptr(), _workspace(self.device).data_ptr(), ptr),
-                  "gp_grad_sum_squares")
+        if stream is not None or self.device.index != _current_device():
+            with _On(self.device, stream):
+                return self.sum_squares()
+        total = torch.empty((), dtype=torch.float64, device=self.device)
+        check(native.lib().gp_grad_sum_squares(self._h, total.data_ptr(), _workspace(self.device).data_ptr(),
+                                               _current_stream(self.device.index)), "gp_grad_sum_squares")
         return total
 
     def norm(self, stream=None) -> torch.Tensor:
@@ -125,10 +127,13 @@ class GradPlan:
         self._open()
         max_norm, scale, mode = _bound(max_norm, scale, skip_nonfinite)
         given = _total(total, self.device)
-        with _On(self.device, stream) as ptr:
-            norm = torch.empty((), dtype=torch.float32, device=self.device)
-            check(native.lib().gp_grad_clip(self._h, max_norm, scale, mode, given, norm.data_ptr(),
-                                            _workspace(self.device).data_ptr(), ptr), "gp_grad_clip")
+        if stream is not None or self.device.index != _current_device():
+            with _On(self.device, stream):
+                return self.clip(max_norm, scale, total, skip_nonfinite)
+        norm = torch.empty((), dtype=torch.float32, device=self.device)
+        check(native.lib().gp_grad_clip(self._h, max_norm, scale, mode, given, norm.data_ptr(),
+                                        _workspace(self.device).data_ptr(), _current_stream(self.device.index)),
+              "gp_grad_clip")
         return norm
 
     def close(self) -> None:
@@ -172,13 +177,15 @@ def sum_updates_squares(updates: Sequence[torch.Tensor], scratch: torch.Tensor |
         raise ValueError("no updates")
     _flat(updates[0], "updates[0]", torch.float32)
     device, n = updates[0].device, updates[0].numel()
+    if stream is not None or device.index != _current_device():
+        with _On(device, stream):
+            return sum_updates_squares(updates, scratch)
     ptrs = _buckets(updates, n, device)
-    with _On(device, stream) as ptr:
-        scratch = _scratch(scratch, len(updates), n, device)
-        total = torch.empty((), dtype=torch.float64, device=device)
-        check(native.lib().gp_bucket_sum_squares(None if scratch is None else scratch.data_ptr(), ptrs, len(updates),
-                                                 n, total.data_ptr(), _workspace(device).data_ptr(), ptr),
-              "gp_bucket_sum_squares")
+    scratch = _scratch(scratch, len(updates), n, device)
+    total = torch.empty((), dtype=torch.float64, device=device)
+    check(native.lib().gp_bucket_sum_squares(None if scratch is None else scratch.data_ptr(), ptrs, len(updates), n,
+                                             total.data_ptr(), _workspace(device).data_ptr(),
+                                             _current_stream(device.index)), "gp_bucket_sum_squares")
     return total
 
 
@@ -193,24 +200,26 @@ def apply_updates_clipped(master: torch.Tensor, updates: Sequence[torch.Tensor],
     ``total``: the sum of squares to go by, over all tables or ranks; u is then
     taken from ``scratch`` as sum_updates_squares left it.  A norm that is infinite
     or NaN goes into the table, or, with ``skip_nonfinite``, leaves it unchanged."""
-    max_norm, scale, mode = _bound(max_norm, scale, skip_nonfinite)
     _flat(master, "master", torch.float32)
     device, n = master.device, master.numel()
+    if stream is not None or device.index != _current_device():
+        with _On(device, stream):
+            return apply_updates_clipped(master, updates, max_norm, scale, out, scratch, total, skip_nonfinite)
     if out is None:
         out = master
     else:
         _flat(out, "out", torch.float32, device)
         if out.numel() < n:
             raise ValueError("out smaller than the master")
+    max_norm, bound_scale, mode = _bound(max_norm, scale, skip_nonfinite)
     ptrs = _buckets(updates, n, device)
     given = _total(total, device)
     if given is not None and scratch is None and len(updates) > 2:
         raise ValueError("total needs the scratch that sum_updates_squares left")
-    with _On(device, stream) as ptr:
-        scratch = _scratch(scratch, len(updates), n, device)
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        check(native.lib().gp_bucket_sum_clipped(out.data_ptr(), master.data_ptr(), ptrs, len(updates), n,
-                                                 None if scratch is None else scratch.data_ptr(), max_norm, scale,
-                                                 mode, given, norm.data_ptr(), _workspace(device).data_ptr(), ptr),
-              "gp_bucket_sum_clipped")
+    scratch = _scratch(scratch, len(updates), n, device)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    check(native.lib().gp_bucket_sum_clipped(out.data_ptr(), master.data_ptr(), ptrs, len(updates), n,
+                                             None if scratch is None else scratch.data_ptr(), max_norm, bound_scale, mode,
+                                             given, norm.data_ptr(), _workspace(device).data_ptr(),
+                                             _current_stream(device.index)), "gp_bucket_sum_clipped")
     return norm

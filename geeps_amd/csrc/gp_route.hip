@@ -50,34 +50,40 @@ __global__ __launch_bounds__(kSortBlock) void route_count_kernel(const I *__rest
   if ((int)threadIdx.x < experts) hist[(size_t)blockIdx.x * experts + threadIdx.x] = count[threadIdx.x];
 }
 
+// A block of W waves.
+template <int W>
 struct SortShared {
-  int run[kSortWaves][kMaxExperts];  // a wave's next place in every expert's group
+  int run[W][kMaxExperts];  // a wave's next place in every expert's group
   int total[kMaxExperts];
   int before[kMaxExperts];  // choices of earlier blocks
   int offset[kMaxExperts + 1];
-  int wave[kSortWaves];
+  int wave[W];
 };
 
-// After it, s.run holds every wave's first places and s.total / s.offset the groups.
-template <typename I>
-__device__ void route_prepare(SortShared &s, const I *__restrict__ ids, unsigned lo, unsigned hi, unsigned per_wave,
-                              int experts, int align, const int *__restrict__ hist, unsigned block,
-                              unsigned blocks) {
+// After it, s.run holds every wave's first places and s.total / s.offset the
+// groups.  `key` is the lane's own first choice, so that a wave with one step
+// reads its ids once.
+template <int W, typename I>
+__device__ __forceinline__ void route_prepare(SortShared<W> &s, int key, const I *__restrict__ ids, unsigned from,
+                                              unsigned to, int experts, int align, const int *__restrict__ hist,
+                                              unsigned block, unsigned blocks) {
+  constexpr int kThreads = W * kWave;
+  constexpr int kPer = kMaxExperts / kThreads;  // experts to a thread, next to each other
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
-  if (tid < experts) {
+  for (int e = tid; e < experts; e += kThreads) {
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) s.run[w][tid] = 0;
-    s.total[tid] = 0;
-    s.before[tid] = 0;
+    for (int w = 0; w < W; ++w) s.run[w][e] = 0;
+    s.total[e] = 0;
+    s.before[e] = 0;
   }
   __syncthreads();
-  const unsigned from = min(hi, lo + wave * per_wave), to = min(hi, from + per_wave);
-  for (unsigned i = from + lane; i < to; i += kWave) {
-    const int key = key_of(ids[i], experts);
-    if (key < experts) atomicAdd(&s.run[wave][key], 1);
+  if (key < experts) atomicAdd(&s.run[wave][key], 1);
+  for (unsigned i = from + kWave + lane; i < to; i += kWave) {
+    const int k = key_of(ids[i], experts);
+    if (k < experts) atomicAdd(&s.run[wave][k], 1);
   }
   if (blocks > 1) {
-    const int parts = kSortBlock / experts;  // >= 1; thread (part, expert) sums every parts-th block's count
+    const int parts = kThreads / experts;  // thread (part, expert) sums every parts-th block's count
     const int e = tid % experts, part = tid / experts;
     if (part < parts) {
       int total = 0, before = 0;
@@ -92,17 +98,24 @@ __device__ void route_prepare(SortShared &s, const I *__restrict__ ids, unsigned
     }
   }
   __syncthreads();
-  int mine = 0;
-  if (tid < experts) {
-    if (blocks == 1) {
+  int padded[kPer], sum = 0;
 #pragma unroll
-      for (int w = 0; w < kSortWaves; ++w) mine += s.run[w][tid];
-      s.total[tid] = mine;
-    } else {
-      mine = s.total[tid];
+  for (int j = 0; j < kPer; ++j) {
+    const int e = tid * kPer + j;
+    int mine = 0;
+    if (e < experts) {
+      if (blocks == 1) {
+#pragma unroll
+        for (int w = 0; w < W; ++w) mine += s.run[w][e];
+        s.total[e] = mine;
+      } else {
+        mine = s.total[e];
+      }
     }
+    padded[j] = align == 1 ? mine : (mine + align - 1) / align * align;
+    sum += padded[j];
   }
-  int padded = (mine + align - 1) / align * align, scan = padded;
+  int scan = sum;
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) {
     const int up = __shfl_up(scan, d, kWave);
@@ -110,16 +123,20 @@ __device__ void route_prepare(SortShared &s, const I *__restrict__ ids, unsigned
   }
   if (lane == kWave - 1) s.wave[wave] = scan;
   __syncthreads();
-  int base = scan - padded;
+  int base = scan - sum;
   for (int w = 0; w < wave; ++w) base += s.wave[w];
-  if (tid < experts) {
-    s.offset[tid] = base;
-    if (tid == experts - 1) s.offset[experts] = base + padded;
-    int at = base + s.before[tid];
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) {
-      const int c = s.run[w][tid];
-      s.run[w][tid] = at;
+  for (int j = 0; j < kPer; ++j) {
+    const int e = tid * kPer + j;
+    if (e >= experts) break;
+    s.offset[e] = base;
+    int at = base + s.before[e];
+    base += padded[j];
+    if (e == experts - 1) s.offset[experts] = base;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const int c = s.run[w][e];
+      s.run[w][e] = at;
       at += c;
     }
   }
@@ -127,7 +144,8 @@ __device__ void route_prepare(SortShared &s, const I *__restrict__ ids, unsigned
 }
 
 // The wave's 64 choices of one step: each lane's place, or -1.
-__device__ __forceinline__ int route_step(SortShared &s, int key, int experts, int bits) {
+template <int W>
+__device__ __forceinline__ int route_step(SortShared<W> &s, int key, int experts, int bits) {
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   uint64_t same = ~0ull;
   for (int b = 0; b < bits; ++b) {
@@ -147,11 +165,13 @@ __global__ __launch_bounds__(kSortBlock) void route_place_kernel(
     const I *__restrict__ ids, unsigned n, unsigned per_block, int experts, int bits, int align, unsigned rows,
     const int *__restrict__ hist, int *__restrict__ position, int *__restrict__ order, int *__restrict__ counts,
     int *__restrict__ offsets) {
-  __shared__ SortShared s;
+  __shared__ SortShared<kSortWaves> s;
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
   const unsigned lo = blockIdx.x * per_block, hi = min(n, lo + per_block);
   const unsigned per_wave = per_block / kSortWaves;
-  route_prepare(s, ids, lo, hi, per_wave, experts, align, hist, blockIdx.x, gridDim.x);
+  const unsigned from = min(hi, lo + wave * per_wave), to = min(hi, from + per_wave);
+  int key = from + lane < to ? key_of(ids[from + lane], experts) : experts;
+  route_prepare(s, key, ids, from, to, experts, align, hist, blockIdx.x, gridDim.x);
   if (blockIdx.x == 0) {
     if (tid < experts) {
       counts[tid] = s.total[tid];
@@ -159,18 +179,18 @@ __global__ __launch_bounds__(kSortBlock) void route_place_kernel(
     }
     if (tid == 0) offsets[experts] = s.offset[experts];
   }
-  const unsigned from = min(hi, lo + wave * per_wave), to = min(hi, from + per_wave);
   for (unsigned i0 = from; i0 < to; i0 += kWave) {
     const unsigned i = i0 + lane;
-    const int key = i < to ? key_of(ids[i], experts) : experts;
+    if (i0 != from) key = i < to ? key_of(ids[i], experts) : experts;
     const int at = route_step(s, key, experts, bits);
     if (i < to) position[i] = at;
     if (at >= 0) order[at] = (int)i;
   }
   // places that hold no choice: the groups' padding, then all behind the last group
   const unsigned waves = gridDim.x * kSortWaves, me = blockIdx.x * kSortWaves + wave;
-  for (unsigned e = me; e < (unsigned)experts; e += waves)
-    for (int p = s.offset[e] + s.total[e] + lane; p < s.offset[e + 1]; p += kWave) order[p] = -1;
+  if (align > 1)
+    for (unsigned e = me; e < (unsigned)experts; e += waves)
+      for (int p = s.offset[e] + s.total[e] + lane; p < s.offset[e + 1]; p += kWave) order[p] = -1;
   for (unsigned p = s.offset[experts] + me * kWave + lane; p < rows; p += waves * kWave) order[p] = -1;
 }
 
@@ -183,32 +203,52 @@ constexpr int kMoveBlock = 256;
 constexpr int kMoveWaves = kMoveBlock / kWave;
 constexpr unsigned kZeroRows = 16;  // places that one wave looks through for rows to clear
 
+// Rows are read and written once, so they go past the caches (non-temporal):
+// 16384 tokens of 4096 bf16, 8 choices: dispatch 209 us, not 242, combine 207,
+// not 240, its gradient 415, not 457.  But not the loads of rows that start off
+// a 16-byte boundary, whose lines two of a wave's accesses share: the gradient
+// of 4099 tokens of 1001 floats took 27 us with them, 22 without.
 struct Shape {
   unsigned tokens, k, rows, width;
   unsigned splits;       // waves that share a token's columns
   unsigned token_waves;  // tokens * splits
 };
 
-// Rows that hold no choice are cleared, kZeroRows places to a wave.
+// Clears row first + lane for every lane that finds it `empty`.
 template <typename E>
-__device__ void clear_rows(E *__restrict__ out, size_t stride, const int *__restrict__ order, const Shape &d,
-                           unsigned wave) {
+__device__ __forceinline__ void clear_rows(E *__restrict__ out, size_t stride, unsigned first, bool empty,
+                                           unsigned width) {
   using V = Vec<E>;
   const int lane = threadIdx.x % kWave;
-  const unsigned first = wave * kZeroRows;
-  const unsigned at = first + lane;
-  const bool mine = lane < (int)kZeroRows && at < d.rows;
-  const int o = mine ? order[at] : 0;
-  uint64_t empty = __ballot(mine && (o < 0 || (unsigned)o >= d.tokens * d.k));
-  while (empty) {
-    E *row = out + (size_t)(first + (__ffsll((long long)empty) - 1)) * stride;
-    empty &= empty - 1;
-    for (unsigned c = lane * V::N; c < d.width; c += kWave * V::N) {
+  for (uint64_t left = __ballot(empty); left; left &= left - 1) {
+    E *row = out + (size_t)(first + (__ffsll((long long)left) - 1)) * stride;
+    for (unsigned c = lane * V::N; c < width; c += kWave * V::N) {
       const typename V::Raw zero = (E)0.0f;
-      if (c + V::N <= d.width)
-        store_raw(row + c, zero);
+      if (c + V::N <= width)
+        store_raw<E, true>(row + c, zero);
       else
-        store_part(row + c, zero, d.width - c);
+        store_part(row + c, zero, width - c);
+    }
+  }
+}
+
+// A token's columns of one wave, to the row of every choice; p: lane c's row.
+template <typename E>
+__device__ __forceinline__ void dispatch_token(E *__restrict__ out, size_t out_stride, const E *__restrict__ from,
+                                               int p, unsigned split, const Shape &d) {
+  using V = Vec<E>;
+  const int lane = threadIdx.x % kWave;
+  const uint64_t held = __ballot((unsigned)p < d.rows);
+  for (unsigned c = (split * kWave + lane) * V::N; c < d.width; c += d.splits * kWave * V::N) {
+    const bool whole = c + V::N <= d.width;
+    const typename V::Raw v = whole ? load_raw(from + c) : load_part(from + c, d.width - c);
+    for (uint64_t left = held; left; left &= left - 1) {
+      const int to = __builtin_amdgcn_readlane(p, __ffsll((long long)left) - 1);
+      E *row = out + (size_t)to * out_stride + c;
+      if (whole)
+        store_raw<E, true>(row, v);
+      else
+        store_part(row, v, d.width - c);
     }
   }
 }
@@ -218,29 +258,82 @@ __global__ __launch_bounds__(kMoveBlock) void route_dispatch_kernel(E *__restric
                                                                     const E *__restrict__ x, size_t x_stride,
                                                                     const int *__restrict__ position,
                                                                     const int *__restrict__ order, Shape d) {
-  using V = Vec<E>;
   const unsigned wave = blockIdx.x * kMoveWaves + threadIdx.x / kWave;
   const int lane = threadIdx.x % kWave;
   if (wave >= d.token_waves) {
-    clear_rows(out, out_stride, order, d, wave - d.token_waves);
+    const unsigned first = (wave - d.token_waves) * kZeroRows, at = first + lane;
+    const bool mine = lane < (int)kZeroRows && at < d.rows;
+    const int o = mine ? order[at] : 0;
+    clear_rows(out, out_stride, first, mine && (o < 0 || (unsigned)o >= d.tokens * d.k), d.width);
     return;
   }
-  const unsigned t = wave / d.splits, split = wave % d.splits;
+  const unsigned t = wave / d.splits;
   const int p = lane < (int)d.k ? position[(size_t)t * d.k + lane] : -1;
-  const uint64_t held = __ballot((unsigned)p < d.rows);
-  const E *from = x + (size_t)t * x_stride;
-  for (unsigned c = (split * kWave + lane) * V::N; c < d.width; c += d.splits * kWave * V::N) {
-    const bool whole = c + V::N <= d.width;
-    const typename V::Raw v = whole ? load_raw(from + c) : load_part(from + c, d.width - c);
-    for (uint64_t left = held; left; left &= left - 1) {
-      const int to = __builtin_amdgcn_readlane(p, __ffsll((long long)left) - 1);
-      E *row = out + (size_t)to * out_stride + c;
-      if (whole)
-        store_raw(row, v);
-      else
-        store_part(row, v, d.width - c);
+  dispatch_token(out, out_stride, x + (size_t)t * x_stride, p, wave % d.splits, d);
+}
+
+// Few choices: every block makes the places for itself, in LDS, and moves its
+// own tokens, in one launch.  The first block leaves the places for later
+// calls.  16 tokens of 4096 bf16, 4 choices: see the host side.
+constexpr unsigned kSmallRoute = 1024;
+
+template <typename E, typename I>
+__global__ __launch_bounds__(kMoveBlock) void route_sort_dispatch_kernel(
+    E *__restrict__ out, size_t out_stride, const E *__restrict__ x, size_t x_stride, const I *__restrict__ ids,
+    int experts, int bits, int align, int *__restrict__ position, int *__restrict__ order, int *__restrict__ counts,
+    int *__restrict__ offsets, Shape d) {
+  __shared__ SortShared<kMoveWaves> s;
+  __shared__ int place[kSmallRoute];
+  const unsigned n = d.tokens * d.k;
+  const int tid = threadIdx.x, in_block = tid / kWave, lane = tid % kWave;
+  const unsigned per_wave = (n + kMoveBlock - 1) / kMoveBlock * kWave;
+  const unsigned from = min(n, in_block * per_wave), to = min(n, from + per_wave);
+  int key = from + lane < to ? key_of(ids[from + lane], experts) : experts;
+  route_prepare(s, key, ids, from, to, experts, align, (const int *)nullptr, 0u, 1u);
+  for (unsigned i0 = from; i0 < to; i0 += kWave) {
+    const unsigned i = i0 + lane;
+    if (i0 != from) key = i < to ? key_of(ids[i], experts) : experts;
+    const int at = route_step(s, key, experts, bits);
+    if (i < to) {
+      place[i] = at;
+      if (blockIdx.x == 0) {
+        position[i] = at;
+        if (at >= 0) order[at] = (int)i;
+      }
     }
   }
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    for (int e = tid; e < experts; e += kMoveBlock) {
+      counts[e] = s.total[e];
+      offsets[e] = s.offset[e];
+    }
+    if (tid == 0) offsets[experts] = s.offset[experts];
+  }
+  const unsigned wave = blockIdx.x * kMoveWaves + in_block;
+  if (wave >= d.token_waves) {
+    // a row's group is the last that starts at or before it; behind the
+    // group's choices the row is empty
+    const unsigned first = (wave - d.token_waves) * kZeroRows, r = first + lane;
+    bool empty = false;
+    if (lane < (int)kZeroRows && r < d.rows) {
+      int lo = 0, hi = experts;  // offset[lo] <= r < offset[hi], or r is behind the last group
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (s.offset[mid] <= (int)r)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      empty = (int)r - s.offset[lo] >= s.total[lo];
+      if (empty) order[r] = -1;
+    }
+    clear_rows(out, out_stride, first, empty, d.width);
+    return;
+  }
+  const unsigned t = wave / d.splits;
+  const int p = lane < (int)d.k ? place[t * d.k + lane] : -1;
+  dispatch_token(out, out_stride, x + (size_t)t * x_stride, p, wave % d.splits, d);
 }
 
 // Weights: none (1), float, or the rows' own type.
@@ -255,7 +348,7 @@ __device__ __forceinline__ float weight_at(const void *w, int type, size_t i) {
 
 // G held choices from `left` on: their rows' 16 bytes are all asked for before
 // the first is used.
-template <typename E, int G>
+template <typename E, int G, bool NT>
 __device__ __forceinline__ void combine_group(typename Vec<E>::F &acc, uint64_t &left, const E *__restrict__ rows,
                                               size_t stride, int p, float w, unsigned c, bool whole, unsigned width) {
   using V = Vec<E>;
@@ -267,13 +360,13 @@ __device__ __forceinline__ void combine_group(typename Vec<E>::F &acc, uint64_t 
     left &= left - 1;
     const E *row = rows + (size_t)__builtin_amdgcn_readlane(p, from) * stride + c;
     f[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), from));
-    v[g] = whole ? load_raw(row) : load_part(row, width - c);
+    v[g] = whole ? load_raw<E, NT>(row) : load_part(row, width - c);
   }
 #pragma unroll
   for (int g = 0; g < G; ++g) acc += f[g] * to_float<E>(v[g]);  // choices in order, in 32 bits
 }
 
-template <typename E>
+template <typename E, bool NT>
 __global__ __launch_bounds__(kMoveBlock) void route_combine_kernel(E *__restrict__ y, size_t y_stride,
                                                                    const E *__restrict__ rows, size_t row_stride,
                                                                    const int *__restrict__ position,
@@ -294,12 +387,12 @@ __global__ __launch_bounds__(kMoveBlock) void route_combine_kernel(E *__restrict
     typename V::F acc = 0.0f;
     uint64_t left = held;
     int n = __popcll(held);
-    for (; n >= 8; n -= 8) combine_group<E, 8>(acc, left, rows, row_stride, p, w, c, whole, d.width);
-    if (n >= 4) combine_group<E, 4>(acc, left, rows, row_stride, p, w, c, whole, d.width), n -= 4;
-    if (n >= 2) combine_group<E, 2>(acc, left, rows, row_stride, p, w, c, whole, d.width), n -= 2;
-    if (n >= 1) combine_group<E, 1>(acc, left, rows, row_stride, p, w, c, whole, d.width);
+    for (; n >= 8; n -= 8) combine_group<E, 8, NT>(acc, left, rows, row_stride, p, w, c, whole, d.width);
+    if (n >= 4) combine_group<E, 4, NT>(acc, left, rows, row_stride, p, w, c, whole, d.width), n -= 4;
+    if (n >= 2) combine_group<E, 2, NT>(acc, left, rows, row_stride, p, w, c, whole, d.width), n -= 2;
+    if (n >= 1) combine_group<E, 1, NT>(acc, left, rows, row_stride, p, w, c, whole, d.width);
     if (whole)
-      store_raw(to + c, from_float<E>(acc));
+      store_raw<E, true>(to + c, from_float<E>(acc));
     else
       store_part(to + c, from_float<E>(acc), d.width - c);
   }
@@ -311,7 +404,7 @@ __global__ __launch_bounds__(kMoveBlock) void route_combine_kernel(E *__restrict
 // are 32-bit sums, lane by lane, then over the wave, then over the splits' waves
 // in their order.
 // ---------------------------------------------------------------------------
-template <typename E, int G>
+template <typename E, int G, bool NT>
 __device__ __forceinline__ void grad_group(uint64_t &left, E *__restrict__ d_rows, size_t d_stride,
                                            const E *__restrict__ dy, const E *__restrict__ rows, size_t row_stride,
                                            int p, float w, unsigned first, unsigned step, unsigned width, float &dot) {
@@ -336,7 +429,7 @@ __device__ __forceinline__ void grad_group(uint64_t &left, E *__restrict__ d_row
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       const E *row = rows + at[g] * row_stride + c;
-      v[g] = whole ? load_raw(row) : load_part(row, part);
+      v[g] = whole ? load_raw<E, NT>(row) : load_part(row, part);
     }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -346,7 +439,7 @@ __device__ __forceinline__ void grad_group(uint64_t &left, E *__restrict__ d_row
       E *row = d_rows + at[g] * d_stride + c;
       const typename V::Raw out = from_float<E>(f[g] * o);
       if (whole)
-        store_raw(row, out);
+        store_raw<E, true>(row, out);
       else
         store_part(row, out, part);
     }
@@ -359,7 +452,7 @@ __device__ __forceinline__ void grad_group(uint64_t &left, E *__restrict__ d_row
 }
 
 // S waves share a token (d.splits = S); a block holds kMoveWaves / S tokens.
-template <typename E, int S>
+template <typename E, int S, bool NT>
 __global__ __launch_bounds__(kMoveBlock) void route_combine_grad_kernel(
     E *__restrict__ d_rows, size_t d_stride, void *__restrict__ d_weights, const E *__restrict__ dy, size_t dy_stride,
     const E *__restrict__ rows, size_t row_stride, const int *__restrict__ position, const int *__restrict__ order,
@@ -371,7 +464,10 @@ __global__ __launch_bounds__(kMoveBlock) void route_combine_grad_kernel(
   const int lane = threadIdx.x % kWave;
   const bool moves = wave < d.token_waves;
   if (!moves) {  // these waves clear, and meet the others at the barrier below
-    clear_rows(d_rows, d_stride, order, d, wave - d.token_waves);
+    const unsigned first = (wave - d.token_waves) * kZeroRows, at = first + lane;
+    const bool look = lane < (int)kZeroRows && at < d.rows;
+    const int o = look ? order[at] : 0;
+    clear_rows(d_rows, d_stride, first, look && (o < 0 || (unsigned)o >= d.tokens * d.k), d.width);
   }
   const unsigned t = wave / S, split = wave % S;
   const size_t a = (size_t)t * d.k + lane;
@@ -385,10 +481,10 @@ __global__ __launch_bounds__(kMoveBlock) void route_combine_grad_kernel(
     const unsigned first = (split * kWave + lane) * V::N, step = S * kWave * V::N;
     uint64_t left = held;
     int n = __popcll(held);
-    for (; n >= 8; n -= 8) grad_group<E, 8>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot);
-    if (n >= 4) grad_group<E, 4>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot), n -= 4;
-    if (n >= 2) grad_group<E, 2>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot), n -= 2;
-    if (n >= 1) grad_group<E, 1>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot);
+    for (; n >= 8; n -= 8) grad_group<E, 8, NT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot);
+    if (n >= 4) grad_group<E, 4, NT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot), n -= 4;
+    if (n >= 2) grad_group<E, 2, NT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot), n -= 2;
+    if (n >= 1) grad_group<E, 1, NT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot);
   }
   if constexpr (S > 1) {
     part[in_block][lane] = dot;
@@ -410,8 +506,13 @@ __global__ __launch_bounds__(kMoveBlock) void route_combine_grad_kernel(
 // ---------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------
-constexpr size_t kSingleSort = 8192;   // choices that one block places
-constexpr size_t kMostSortBlocks = 256;
+// One block places up to 4096 choices (4.8 us at 2048 and 6.9 at 4096, against
+// 6.2 and 6.3 of two launches, which cost the caller another 3).  Above, a
+// block takes 1024, one step to a wave, until the counts that every block
+// sums grow past 12288 (blocks * experts); 131072 choices of 128 experts: 11.5
+// us at 128 blocks, 10.3 at 64, 11.3 at 32; of 512: 25.5, 18.0, 16.1.
+constexpr size_t kSingleSort = 4096;
+constexpr size_t kMostSortCounts = 12288;
 
 struct SortPlan {
   unsigned blocks, per_block;
@@ -421,8 +522,9 @@ struct SortPlan {
 SortPlan sort_plan(size_t n, size_t experts) {
   SortPlan p;
   const size_t unit = kSortBlock;  // every wave takes whole steps of 64
-  size_t per = n <= kSingleSort ? n : 4 * unit;
-  if (n > kSingleSort && (n + per - 1) / per > kMostSortBlocks) per = (n + kMostSortBlocks - 1) / kMostSortBlocks;
+  const size_t most = kMostSortCounts / experts < 256 ? kMostSortCounts / experts : 256;  // 12 at least
+  size_t per = n;
+  if (n > kSingleSort) per = (n + most - 1) / most;
   per = per ? (per + unit - 1) / unit * unit : unit;
   p.per_block = (unsigned)per;
   p.blocks = (unsigned)((n + per - 1) / per);
@@ -455,15 +557,21 @@ int check_move(size_t tokens, size_t k, size_t rows, size_t width, int type) {
   return GP_OK;
 }
 
-// Waves over a token's columns: enough of them to fill the chip when tokens
-// are few, one when tokens alone do.
+// Waves over a token's columns.  Eight, where there are as many steps of 64
+// lanes, keep a row's accesses together in time (8192 tokens of 2048 bf16, 8
+// choices: dispatch 52 us, 64 with 2 waves); more when tokens are few, until
+// the chip has 4 waves per SIMD.
 unsigned pick_splits(size_t tokens, size_t width, int type) {
   const size_t per_step = kWave * 16 / type_size(type);
   const size_t steps = (width + per_step - 1) / per_step;
-  const size_t want = (size_t)device_cus() * 16;  // 4 waves per SIMD
+  const size_t want = (size_t)device_cus() * 16;
   size_t s = tokens ? want / tokens : 1;
-  if (s < 1) s = 1;
+  if (s < 8) s = 8;
   return (unsigned)(s < steps ? s : (steps ? steps : 1));
+}
+
+bool rows_aligned(const void *p, size_t stride, int type) {
+  return ((reinterpret_cast<uintptr_t>(p) | stride * type_size(type)) & 15) == 0;
 }
 
 int check_grid(size_t waves, unsigned *blocks) {
@@ -503,6 +611,21 @@ void launch_sort(const void *ids, const SortPlan &p, size_t n, int experts, int 
 
 size_t strided_bytes(size_t rows, size_t stride, size_t width, int type) {
   return rows && width ? ((rows - 1) * stride + width) * type_size(type) : 0;
+}
+
+int plan_dispatch(const void *out, size_t out_stride, const void *x, size_t x_stride, int type, size_t tokens,
+                  size_t k, size_t rows, size_t width, Shape *d, unsigned *blocks) {
+  GP_TRY(check_move(tokens, k, rows, width, type));
+  GP_REQUIRE(out && (tokens == 0 || x), "null out or x");
+  GP_REQUIRE(out_stride >= width && x_stride >= width, "row stride smaller than the width");
+  GP_REQUIRE(!bytes_overlap(out, strided_bytes(rows, out_stride, width, type), x,
+                            strided_bytes(tokens, x_stride, width, type)),
+             "out overlaps x");
+  *d = Shape{(unsigned)tokens, (unsigned)k, (unsigned)rows, (unsigned)width, pick_splits(tokens, width, type), 0};
+  const size_t waves = tokens * (size_t)d->splits;
+  GP_TRY(check_grid(waves + (rows + kZeroRows - 1) / kZeroRows, blocks));
+  d->token_waves = (unsigned)waves;
+  return GP_OK;
 }
 
 }  // namespace
@@ -554,20 +677,47 @@ int gp_route_dispatch(void *out, size_t out_stride, const void *x, size_t x_stri
                       size_t width, gp_stream s) {
   GP_TRY(check_move(tokens, k, rows, width, type));
   if (rows == 0 || width == 0) return GP_OK;
-  GP_REQUIRE(out && order && (tokens == 0 || (x && position)), "null out, x, position or order");
-  GP_REQUIRE(out_stride >= width && x_stride >= width, "row stride smaller than the width");
-  GP_REQUIRE(!bytes_overlap(out, strided_bytes(rows, out_stride, width, type), x,
-                            strided_bytes(tokens, x_stride, width, type)),
-             "out overlaps x");
-  Shape d{(unsigned)tokens, (unsigned)k, (unsigned)rows, (unsigned)width, pick_splits(tokens, width, type), 0};
-  const size_t waves = tokens * (size_t)d.splits;
+  GP_REQUIRE(order && (tokens == 0 || position), "null position or order");
+  Shape d;
   unsigned blocks = 0;
-  GP_TRY(check_grid(waves + (rows + kZeroRows - 1) / kZeroRows, &blocks));
-  d.token_waves = (unsigned)waves;
+  GP_TRY(plan_dispatch(out, out_stride, x, x_stride, type, tokens, k, rows, width, &d, &blocks));
   with_type(type, [&](auto e) {
     using E = decltype(e);
     hipLaunchKernelGGL((route_dispatch_kernel<E>), dim3(blocks), dim3(kMoveBlock), 0, (hipStream_t)s,
                        static_cast<E *>(out), out_stride, static_cast<const E *>(x), x_stride, position, order, d);
+  });
+  GP_HIP_TRY(hipGetLastError());
+  return GP_OK;
+}
+
+int gp_route_sort_dispatch(void *out, size_t out_stride, const void *x, size_t x_stride, int type, const void *ids,
+                           int id_bits, size_t tokens, size_t k, size_t experts, size_t align, size_t width,
+                           int32_t *position, int32_t *order, int32_t *counts, int32_t *offsets, void *workspace,
+                           size_t workspace_bytes, gp_stream s) {
+  GP_TRY(check_groups(tokens, k, experts, align));
+  const size_t rows = grouped_rows(tokens, k, experts, align), n = tokens * k;
+  if (n == 0 || n > kSmallRoute || width == 0) {
+    GP_TRY(check_move(tokens, k, rows, width, type));
+    GP_TRY(gp_route_sort(ids, id_bits, tokens, k, experts, align, position, order, counts, offsets, workspace,
+                         workspace_bytes, s));
+    return gp_route_dispatch(out, out_stride, x, x_stride, type, position, order, tokens, k, rows, width, s);
+  }
+  GP_REQUIRE(id_bits == 32 || id_bits == 64, "ids must be 32 or 64 bits wide");
+  GP_REQUIRE(ids && position && order && counts && offsets, "null ids, position, order, counts or offsets");
+  Shape d;
+  unsigned blocks = 0;
+  GP_TRY(plan_dispatch(out, out_stride, x, x_stride, type, tokens, k, rows, width, &d, &blocks));
+  const SortPlan p = sort_plan(n, experts);
+  with_type(type, [&](auto e) {
+    using E = decltype(e);
+    auto go = [&](auto id) {
+      using I = decltype(id);
+      hipLaunchKernelGGL((route_sort_dispatch_kernel<E, I>), dim3(blocks), dim3(kMoveBlock), 0, (hipStream_t)s,
+                         static_cast<E *>(out), out_stride, static_cast<const E *>(x), x_stride,
+                         static_cast<const I *>(ids), (int)experts, p.bits, (int)align, position, order, counts,
+                         offsets, d);
+    };
+    id_bits == 64 ? go((int64_t)0) : go((int32_t)0);
   });
   GP_HIP_TRY(hipGetLastError());
   return GP_OK;
@@ -592,9 +742,14 @@ int gp_route_combine(void *y, size_t y_stride, const void *rows_in, size_t row_s
   d.token_waves = (unsigned)waves;
   with_type(type, [&](auto e) {
     using E = decltype(e);
-    hipLaunchKernelGGL((route_combine_kernel<E>), dim3(blocks), dim3(kMoveBlock), 0, (hipStream_t)s,
-                       static_cast<E *>(y), y_stride, static_cast<const E *>(rows_in), row_stride, position, weights,
-                       wt, d);
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kMoveBlock), 0, (hipStream_t)s, static_cast<E *>(y), y_stride,
+                         static_cast<const E *>(rows_in), row_stride, position, weights, wt, d);
+    };
+    if (rows_aligned(rows_in, row_stride, type))
+      go(route_combine_kernel<E, true>);
+    else
+      go(route_combine_kernel<E, false>);
   });
   GP_HIP_TRY(hipGetLastError());
   return GP_OK;
@@ -617,7 +772,12 @@ int gp_route_combine_grad(void *d_rows, size_t d_stride, void *d_weights, const 
   GP_REQUIRE(!bytes_overlap(d_rows, db, dy, yb), "d_rows overlaps dy");
   GP_REQUIRE(!bytes_overlap(d_rows, db, rows_in, rb), "d_rows overlaps the rows");
   const int wt = weight_type == GP_F32 ? kFloatWeights : kRowWeights;
-  const unsigned splits = pick_splits(tokens, width, type) > 1 ? 4 : 1;
+  // a token's waves meet for its weights' gradients: four, a block, or one.
+  // Short rows off a 16-byte boundary go to one wave (1001 floats: 22 us, 27
+  // with four), as do rows of one step.
+  const bool aligned = rows_aligned(rows_in, row_stride, type);
+  const size_t step = kWave * 16 / type_size(type);
+  const unsigned splits = width <= step || (!aligned && width <= 4 * step && tokens >= 4096) ? 1 : 4;
   Shape d{(unsigned)tokens, (unsigned)k, (unsigned)rows, (unsigned)width, splits, 0};
   const size_t waves = tokens * (size_t)d.splits;
   unsigned blocks = 0;
@@ -631,9 +791,9 @@ int gp_route_combine_grad(void *d_rows, size_t d_stride, void *d_weights, const 
                          position, order, weights, wt, d);
     };
     if (splits == 4)
-      go(route_combine_grad_kernel<E, 4>);
+      aligned ? go(route_combine_grad_kernel<E, 4, true>) : go(route_combine_grad_kernel<E, 4, false>);
     else
-      go(route_combine_grad_kernel<E, 1>);
+      aligned ? go(route_combine_grad_kernel<E, 1, true>) : go(route_combine_grad_kernel<E, 1, false>);
   });
   GP_HIP_TRY(hipGetLastError());
   return GP_OK;

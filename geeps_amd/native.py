@@ -112,6 +112,8 @@ _SIGNATURES = {
     "gp_route_workspace": (_i, [_sz, _sz, _sz, _c.POINTER(_sz)]),
     "gp_route_sort": (_i, [_vp, _i, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "gp_route_dispatch": (_i, [_vp, _sz, _vp, _sz, _i, _vp, _vp, _sz, _sz, _sz, _sz, _vp]),
+    "gp_route_sort_dispatch": (_i, [_vp, _sz, _vp, _sz, _i, _vp, _i, _sz, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _vp,
+                                    _vp, _sz, _vp]),
     "gp_route_combine": (_i, [_vp, _sz, _vp, _sz, _i, _vp, _vp, _i, _sz, _sz, _sz, _sz, _vp]),
     "gp_route_combine_grad": (_i, [_vp, _sz, _vp, _vp, _sz, _vp, _sz, _i, _vp, _vp, _vp, _i, _sz, _sz, _sz,
                                    _sz, _vp]),

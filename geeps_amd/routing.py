@@ -48,28 +48,27 @@ class Route(NamedTuple):
     offsets: torch.Tensor   # (experts + 1,): first row of an expert's group; the end of the last
 
 
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream  # (device index) -> hipStream_t, without a Stream object
+
+
 class _On:
-    """The device and stream of a call: temporaries and outputs are allocated on
-    the stream that uses them."""
+    """The device and stream of a call as the current ones, so that its outputs and
+    temporaries are allocated on the stream that uses them.  The calls below enter
+    it, and call themselves again, unless both are current already."""
 
     def __init__(self, device, stream):
-        self.guard = []
-        if device.index is not None and device.index != torch.cuda.current_device():
-            self.guard.append(torch.cuda.device(device))
-        if stream is None:
-            self.ptr = torch.cuda.current_stream(device).cuda_stream
-        else:
+        self.guard = [torch.cuda.device(device)]
+        if stream is not None:
             if not hasattr(stream, "cuda_stream"):
                 stream = torch.cuda.ExternalStream(int(stream), device=device)
             if stream.device != device:
                 raise ValueError("stream of another device than the tensors")
-            self.ptr = stream.cuda_stream
             self.guard.append(torch.cuda.stream(stream))
 
     def __enter__(self):
         for g in self.guard:
             g.__enter__()
-        return self.ptr
 
     def __exit__(self, *exc):
         for g in reversed(self.guard):
@@ -155,21 +154,15 @@ def group_rows(tokens: int, k: int, num_experts: int, align: int = 1) -> int:
     return rows // align * align
 
 
-def _new_route(tokens, k, rows, num_experts, device) -> Route:
-    return Route(torch.empty((tokens, k), dtype=torch.int32, device=device),
-                 torch.empty(rows, dtype=torch.int32, device=device),
-                 torch.empty(num_experts, dtype=torch.int32, device=device),
-                 torch.empty(num_experts + 1, dtype=torch.int32, device=device))
-
-
-def _sort(expert_ids, tokens, k, num_experts, align, route, ptr) -> None:
+def _new_route(tokens, k, rows, num_experts, device):
+    """The route's tensors and the sort's workspace, of one allocation."""
     need = ctypes.c_size_t()
     check(native.lib().gp_route_workspace(tokens, k, num_experts, ctypes.byref(need)), "gp_route_workspace")
-    scratch = torch.empty(need.value, dtype=torch.uint8, device=expert_ids.device) if need.value else None
-    check(native.lib().gp_route_sort(expert_ids.data_ptr(), 8 * expert_ids.element_size(), tokens, k, num_experts,
-                                     align, route.position.data_ptr(), route.order.data_ptr(),
-                                     route.counts.data_ptr(), route.offsets.data_ptr(),
-                                     scratch.data_ptr() if need.value else None, need.value, ptr), "gp_route_sort")
+    sizes = (tokens * k, rows, num_experts, num_experts + 1)
+    if need.value:
+        sizes += (need.value // 4,)
+    parts = torch.empty(sum(sizes), dtype=torch.int32, device=device).split_with_sizes(sizes)
+    return (Route(parts[0].view(tokens, k), *parts[1:4]), parts[4].data_ptr() if need.value else None, need.value)
 
 
 def sort_tokens(expert_ids: torch.Tensor, num_experts: int, align: int = 1, stream=None) -> Route:
@@ -177,9 +170,15 @@ def sort_tokens(expert_ids: torch.Tensor, num_experts: int, align: int = 1, stre
     expert, tokens in order inside a group, every group rounded up to whole
     multiples of ``align`` rows."""
     tokens, k, rows = _ids(expert_ids, num_experts, align)
-    with _On(expert_ids.device, stream) as ptr:
-        route = _new_route(tokens, k, rows, num_experts, expert_ids.device)
-        _sort(expert_ids, tokens, k, num_experts, align, route, ptr)
+    device = expert_ids.device
+    if stream is not None or device.index != _current_device():
+        with _On(device, stream):
+            return sort_tokens(expert_ids, num_experts, align)
+    route, scratch, size = _new_route(tokens, k, rows, num_experts, device)
+    check(native.lib().gp_route_sort(expert_ids.data_ptr(), 8 * expert_ids.element_size(), tokens, k, num_experts,
+                                     align, route.position.data_ptr(), route.order.data_ptr(),
+                                     route.counts.data_ptr(), route.offsets.data_ptr(), scratch, size,
+                                     _current_stream(device.index)), "gp_route_sort")
     return route
 
 
@@ -187,35 +186,44 @@ def dispatch(x: torch.Tensor, route: Route, out: torch.Tensor | None = None, str
     """``rows[r] = x[route.order[r] // k]``, zeros where a row holds no choice.
     With ``out`` given, its rows behind the layout are left as they were."""
     stride = _rows2d(x, "x")
-    tokens, k, rows = _route(route, x.device)
+    device = x.device
+    tokens, k, rows = _route(route, device)
     if x.shape[0] != tokens:
         raise ValueError(f"x has {x.shape[0]} rows, the route {tokens} tokens")
+    if stream is not None or device.index != _current_device():
+        with _On(device, stream):
+            return dispatch(x, route, out)
     width = x.shape[1]
-    with _On(x.device, stream) as ptr:
-        out, out_stride = _out(out, "out", (rows, width), x)
-        check(native.lib().gp_route_dispatch(out.data_ptr(), out_stride, x.data_ptr(), stride, _TYPES[x.dtype],
-                                             route.position.data_ptr(), route.order.data_ptr(), tokens, k, rows,
-                                             width, ptr), "gp_route_dispatch")
+    out, out_stride = _out(out, "out", (rows, width), x)
+    check(native.lib().gp_route_dispatch(out.data_ptr(), out_stride, x.data_ptr(), stride, _TYPES[x.dtype],
+                                         route.position.data_ptr(), route.order.data_ptr(), tokens, k, rows, width,
+                                         _current_stream(device.index)), "gp_route_dispatch")
     return out
 
 
 def sort_and_dispatch(x: torch.Tensor, expert_ids: torch.Tensor, num_experts: int, align: int = 1,
                       out: torch.Tensor | None = None, stream=None) -> tuple[torch.Tensor, Route]:
-    """``sort_tokens`` and ``dispatch`` in one call: (rows, route)."""
+    """``sort_tokens`` and ``dispatch`` in one call (one launch for few choices):
+    (rows, route)."""
     stride = _rows2d(x, "x")
     tokens, k, rows = _ids(expert_ids, num_experts, align)
-    if x.device != expert_ids.device:
+    device = x.device
+    if device != expert_ids.device:
         raise ValueError("x is on another device")
     if x.shape[0] != tokens:
         raise ValueError(f"x has {x.shape[0]} rows, expert_ids {tokens} tokens")
+    if stream is not None or device.index != _current_device():
+        with _On(device, stream):
+            return sort_and_dispatch(x, expert_ids, num_experts, align, out)
     width = x.shape[1]
-    with _On(x.device, stream) as ptr:
-        route = _new_route(tokens, k, rows, num_experts, x.device)
-        out, out_stride = _out(out, "out", (rows, width), x)
-        _sort(expert_ids, tokens, k, num_experts, align, route, ptr)
-        check(native.lib().gp_route_dispatch(out.data_ptr(), out_stride, x.data_ptr(), stride, _TYPES[x.dtype],
-                                             route.position.data_ptr(), route.order.data_ptr(), tokens, k, rows,
-                                             width, ptr), "gp_route_dispatch")
+    route, scratch, size = _new_route(tokens, k, rows, num_experts, device)
+    out, out_stride = _out(out, "out", (rows, width), x)
+    check(native.lib().gp_route_sort_dispatch(out.data_ptr(), out_stride, x.data_ptr(), stride, _TYPES[x.dtype],
+                                              expert_ids.data_ptr(), 8 * expert_ids.element_size(), tokens, k,
+                                              num_experts, align, width, route.position.data_ptr(),
+                                              route.order.data_ptr(), route.counts.data_ptr(),
+                                              route.offsets.data_ptr(), scratch, size,
+                                              _current_stream(device.index)), "gp_route_sort_dispatch")
     return out, route
 
 
@@ -236,17 +244,20 @@ def combine(rows: torch.Tensor, route: Route, weights: torch.Tensor | None = Non
     token with none gets zeros.  ``weights`` (tokens, k) are float32 or of the
     rows' type; without them every weight is 1."""
     stride = _rows2d(rows, "rows")
-    tokens, k, n = _route(route, rows.device)
+    device = rows.device
+    tokens, k, n = _route(route, device)
     if rows.shape[0] < n:
         raise ValueError(f"rows has {rows.shape[0]} rows, the route {n}")
-    width = rows.shape[1]
     wtype = native.GP_F32 if weights is None else _weights(weights, tokens, k, rows)
-    with _On(rows.device, stream) as ptr:
-        out, out_stride = _out(out, "out", (tokens, width), rows)
-        check(native.lib().gp_route_combine(out.data_ptr(), out_stride, rows.data_ptr(), stride, _TYPES[rows.dtype],
-                                            route.position.data_ptr(),
-                                            None if weights is None else weights.data_ptr(), wtype, tokens, k, n,
-                                            width, ptr), "gp_route_combine")
+    if stream is not None or device.index != _current_device():
+        with _On(device, stream):
+            return combine(rows, route, weights, out)
+    width = rows.shape[1]
+    out, out_stride = _out(out, "out", (tokens, width), rows)
+    check(native.lib().gp_route_combine(out.data_ptr(), out_stride, rows.data_ptr(), stride, _TYPES[rows.dtype],
+                                        route.position.data_ptr(), None if weights is None else weights.data_ptr(),
+                                        wtype, tokens, k, n, width, _current_stream(device.index)),
+          "gp_route_combine")
     return out
 
 
@@ -269,14 +280,17 @@ def combine_grad(dy: torch.Tensor, rows: torch.Tensor, route: Route, weights: to
         raise ValueError(f"dy has {dy.shape[0]} rows, the route {tokens} tokens")
     if rows.shape[0] < n:
         raise ValueError(f"rows has {rows.shape[0]} rows, the route {n}")
-    width = dy.shape[1]
     wtype = _weights(weights, tokens, k, dy)
-    with _On(dy.device, stream) as ptr:
-        out, out_stride = _out(out, "out", (n, width), dy)
-        d_weights = torch.empty_like(weights)
-        check(native.lib().gp_route_combine_grad(out.data_ptr(), out_stride, d_weights.data_ptr(), dy.data_ptr(),
-                                                 dy_stride, rows.data_ptr(), row_stride, _TYPES[dy.dtype],
-                                                 route.position.data_ptr(), route.order.data_ptr(),
-                                                 weights.data_ptr(), wtype, tokens, k, n, width, ptr),
-              "gp_route_combine_grad")
+    device = dy.device
+    if stream is not None or device.index != _current_device():
+        with _On(device, stream):
+            return combine_grad(dy, rows, route, weights, out)
+    width = dy.shape[1]
+    out, out_stride = _out(out, "out", (n, width), dy)
+    d_weights = torch.empty_like(weights)
+    check(native.lib().gp_route_combine_grad(out.data_ptr(), out_stride, d_weights.data_ptr(), dy.data_ptr(),
+                                             dy_stride, rows.data_ptr(), row_stride, _TYPES[dy.dtype],
+                                             route.position.data_ptr(), route.order.data_ptr(), weights.data_ptr(),
+                                             wtype, tokens, k, n, width, _current_stream(device.index)),
+          "gp_route_combine_grad")
     return out, d_weights

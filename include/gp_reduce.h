@@ -396,6 +396,12 @@ int gp_route_sort(const void *ids, int id_bits, size_t tokens, size_t k, size_t 
 int gp_route_dispatch(void *out, size_t out_stride, const void *x, size_t x_stride, int type,
                       const int32_t *position, const int32_t *order, size_t tokens, size_t k, size_t rows,
                       size_t width, gp_stream s);
+/* gp_route_sort, then gp_route_dispatch of the gp_route_rows() rows: one launch
+ * up to 1024 choices. */
+int gp_route_sort_dispatch(void *out, size_t out_stride, const void *x, size_t x_stride, int type, const void *ids,
+                           int id_bits, size_t tokens, size_t k, size_t experts, size_t align, size_t width,
+                           int32_t *position, int32_t *order, int32_t *counts, int32_t *offsets, void *workspace,
+                           size_t workspace_bytes, gp_stream s);
 /* y[t] = sum over c of weights[t * k + c] * rows_in[position[t * k + c]],
  * choices in order, those without a row left out (a token with none: zeros).
  * weights: GP_F32 or the rows' type; NULL: 1 each, which is the gradient of

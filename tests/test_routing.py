@@ -420,3 +420,26 @@ def test_refusals(dev):
         routing.combine(both[:16], route, w, out=both[10:18])
     with pytest.raises(native.GpError, match="overlaps"):
         routing.combine_grad(x, rows, route, w, out=rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("id_type", [torch.int32, torch.int64])
+@pytest.mark.parametrize("tokens,k,experts,align,width", [
+    (0, 3, 5, 4, 16), (1, 1, 1024, 64, 40), (16, 64, 64, 1, 24), (128, 8, 1024, 3, 9), (205, 5, 300, 16, 130),
+    (1024, 1, 3, 8, 8), (1025, 1, 3, 8, 8), (40, 2, 7, 1, 0)])
+def test_sort_and_dispatch_few_choices(dev, id_type, tokens, k, experts, align, width):
+    """The one-launch form up to 1024 choices and the first sizes past it."""
+    r = np.random.default_rng(tokens)
+    for kind in ("any", "one", "none"):
+        ids = r.integers(-2, experts + 2, (tokens, k)) if kind == "any" else np.full((tokens, k), 0 if kind == "one" else -1)
+        want = places(np.where((ids >= 0) & (ids < experts), ids, -1), experts, align)
+        x = as_device((tokens, width), torch.bfloat16, dev, 1)
+        out = as_device((len(want[1]) + 5, width), torch.bfloat16, dev, 2)
+        tail = out[len(want[1]):].clone()
+        rows, route = routing.sort_and_dispatch(x, torch.from_numpy(ids).to(id_type).to(dev), experts, align, out=out)
+        assert rows is out and torch.equal(out[len(want[1]):], tail)
+        same_route(route, want)
+        assert torch.equal(out[:len(want[1])], routing.dispatch(x, route))
+        held = route.order >= 0
+        assert torch.equal(out[:len(want[1])][held], x[route.order[held].long() // k])
+        assert not bool(out[:len(want[1])][~held].any())
