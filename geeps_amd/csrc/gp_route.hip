@@ -24,10 +24,10 @@ constexpr int kMaxChoices = kWave; // a token's choices lie in one wave's lanes
 // A block takes `per_block` choices in a row, a wave per_block / 16 of them, 64
 // at a step.  Within a step, lanes with the same id find each other by one
 // ballot per bit of the id; a lane's rank is the number of such lanes below
-// it, and the first of them moves the wave's own counter in LDS.  With one
-// block the counts of its waves are all there is; with more, route_count_kernel
-// has left every block's counts, and each block sums those before it.  Integer
-// sums only: the places do not depend on any order of arrival.
+// it, and the first of them moves the wave's own counter in LDS.  What lies
+// before the block comes from the block's own count of all choices, or, where
+// these are many, from the counts that route_count_kernel has left of every
+// block.  Integer sums only: the places do not depend on any order of arrival.
 // ---------------------------------------------------------------------------
 template <typename I>
 __device__ __forceinline__ int key_of(I id, int experts) {
@@ -61,12 +61,12 @@ struct SortShared {
 };
 
 // After it, s.run holds every wave's first places and s.total / s.offset the
-// groups.  `key` is the lane's own first choice, so that a wave with one step
+// groups.  lo: the block's first choice; hist: NULL to count all n.  `key` is the lane's own first choice, so that a wave with one step
 // reads its ids once.
 template <int W, typename I>
-__device__ __forceinline__ void route_prepare(SortShared<W> &s, int key, const I *__restrict__ ids, unsigned from,
-                                              unsigned to, int experts, int align, const int *__restrict__ hist,
-                                              unsigned block, unsigned blocks) {
+__device__ __forceinline__ void route_prepare(SortShared<W> &s, int key, const I *__restrict__ ids, unsigned n,
+                                              unsigned lo, unsigned from, unsigned to, int experts, int align,
+                                              const int *__restrict__ hist, unsigned block, unsigned blocks) {
   constexpr int kThreads = W * kWave;
   constexpr int kPer = kMaxExperts / kThreads;  // experts to a thread, next to each other
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
@@ -82,18 +82,24 @@ __device__ __forceinline__ void route_prepare(SortShared<W> &s, int key, const I
     const int k = key_of(ids[i], experts);
     if (k < experts) atomicAdd(&s.run[wave][k], 1);
   }
-  if (blocks > 1) {
+  if (blocks > 1 && !hist) {
+    for (unsigned i = tid; i < n; i += kThreads) {
+      const int k = key_of(ids[i], experts);
+      if (k >= experts) continue;
+      atomicAdd(i < lo ? &s.before[k] : &s.total[k], 1);
+    }
+  } else if (blocks > 1) {
     const int parts = kThreads / experts;  // thread (part, expert) sums every parts-th block's count
     const int e = tid % experts, part = tid / experts;
     if (part < parts) {
-      int total = 0, before = 0;
+      int rest = 0, before = 0;
 #pragma unroll 8
       for (unsigned g = part; g < blocks; g += parts) {
         const int c = hist[(size_t)g * experts + e];
-        total += c;
+        rest += g < block ? 0 : c;
         before += g < block ? c : 0;
       }
-      atomicAdd(&s.total[e], total);
+      atomicAdd(&s.total[e], rest);
       atomicAdd(&s.before[e], before);
     }
   }
@@ -107,10 +113,10 @@ __device__ __forceinline__ void route_prepare(SortShared<W> &s, int key, const I
       if (blocks == 1) {
 #pragma unroll
         for (int w = 0; w < W; ++w) mine += s.run[w][e];
-        s.total[e] = mine;
       } else {
-        mine = s.total[e];
+        mine = s.total[e] + s.before[e];
       }
+      s.total[e] = mine;
     }
     padded[j] = align == 1 ? mine : (mine + align - 1) / align * align;
     sum += padded[j];
@@ -171,7 +177,7 @@ __global__ __launch_bounds__(kSortBlock) void route_place_kernel(
   const unsigned per_wave = per_block / kSortWaves;
   const unsigned from = min(hi, lo + wave * per_wave), to = min(hi, from + per_wave);
   int key = from + lane < to ? key_of(ids[from + lane], experts) : experts;
-  route_prepare(s, key, ids, from, to, experts, align, hist, blockIdx.x, gridDim.x);
+  route_prepare(s, key, ids, n, lo, from, to, experts, align, hist, blockIdx.x, gridDim.x);
   if (blockIdx.x == 0) {
     if (tid < experts) {
       counts[tid] = s.total[tid];
@@ -289,7 +295,7 @@ __global__ __launch_bounds__(kMoveBlock) void route_sort_dispatch_kernel(
   const unsigned per_wave = (n + kMoveBlock - 1) / kMoveBlock * kWave;
   const unsigned from = min(n, in_block * per_wave), to = min(n, from + per_wave);
   int key = from + lane < to ? key_of(ids[from + lane], experts) : experts;
-  route_prepare(s, key, ids, from, to, experts, align, (const int *)nullptr, 0u, 1u);
+  route_prepare(s, key, ids, n, 0u, from, to, experts, align, (const int *)nullptr, 0u, 1u);
   for (unsigned i0 = from; i0 < to; i0 += kWave) {
     const unsigned i = i0 + lane;
     if (i0 != from) key = i < to ? key_of(ids[i], experts) : experts;
@@ -506,26 +512,30 @@ __global__ __launch_bounds__(kMoveBlock) void route_combine_grad_kernel(
 // ---------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------
-// One block places up to 4096 choices (4.8 us at 2048 and 6.9 at 4096, against
-// 6.2 and 6.3 of two launches, which cost the caller another 3).  Above, a
-// block takes 1024, one step to a wave, until the counts that every block
-// sums grow past 12288 (blocks * experts); 131072 choices of 128 experts: 11.5
-// us at 128 blocks, 10.3 at 64, 11.3 at 32; of 512: 25.5, 18.0, 16.1.
-constexpr size_t kSingleSort = 4096;
-constexpr size_t kMostSortCounts = 12288;
+// Up to this many choices every block counts them all for itself: one launch
+// (4.6 us at 4096 choices, 5.5 at 8192, 7.2 at 16384, against 6.3, 6.7 and 7.3
+// of two launches, the second of which costs the caller 3 more).
+constexpr size_t kSelfCounted = 16384;
+// Above, b blocks cost about 1.2 us for each of their n / (1024 b) steps and
+// 2.6e-4 us for each of the b * experts counts that every block sums: least at
+// b * b = 4.4 n / experts.  131072 choices of 512 experts: 25.5 us at 128
+// blocks, 18.0 at 64, 16.1 at 32; of 128: 11.5, 10.3, 11.3.
+constexpr size_t kMostSortBlocks = 1024;
 
 struct SortPlan {
   unsigned blocks, per_block;
+  bool counted;  // by route_count_kernel
   int bits;
 };
 
 SortPlan sort_plan(size_t n, size_t experts) {
   SortPlan p;
   const size_t unit = kSortBlock;  // every wave takes whole steps of 64
-  const size_t most = kMostSortCounts / experts < 256 ? kMostSortCounts / experts : 256;  // 12 at least
-  size_t per = n;
-  if (n > kSingleSort) per = (n + most - 1) / most;
-  per = per ? (per + unit - 1) / unit * unit : unit;
+  size_t most = 1;
+  while (most < kMostSortBlocks && (most + 1) * (most + 1) * experts <= 4 * n + n / 2) ++most;
+  size_t per = n > kSelfCounted ? (n + most - 1) / most : unit;
+  per = (per + unit - 1) / unit * unit;
+  p.counted = n > kSelfCounted;
   p.per_block = (unsigned)per;
   p.blocks = (unsigned)((n + per - 1) / per);
   p.bits = 1;
@@ -602,11 +612,11 @@ template <typename I>
 void launch_sort(const void *ids, const SortPlan &p, size_t n, int experts, int align, size_t rows, int *position,
                  int *order, int *counts, int *offsets, int *hist, hipStream_t s) {
   const I *in = static_cast<const I *>(ids);
-  if (p.blocks > 1)
+  if (p.counted)
     hipLaunchKernelGGL((route_count_kernel<I>), dim3(p.blocks), dim3(kSortBlock), 0, s, in, (unsigned)n, p.per_block,
                        experts, hist);
   hipLaunchKernelGGL((route_place_kernel<I>), dim3(p.blocks), dim3(kSortBlock), 0, s, in, (unsigned)n, p.per_block,
-                     experts, p.bits, align, (unsigned)rows, (const int *)hist, position, order, counts, offsets);
+                     experts, p.bits, align, (unsigned)rows, p.counted ? (const int *)hist : nullptr, position, order, counts, offsets);
 }
 
 size_t strided_bytes(size_t rows, size_t stride, size_t width, int type) {
@@ -643,7 +653,7 @@ int gp_route_workspace(size_t tokens, size_t k, size_t experts, size_t *bytes) {
   GP_REQUIRE(bytes, "null bytes");
   GP_TRY(check_groups(tokens, k, experts, 1));
   const SortPlan p = sort_plan(tokens * k, experts);
-  *bytes = p.blocks > 1 ? (size_t)p.blocks * experts * sizeof(int) : 0;
+  *bytes = p.counted ? (size_t)p.blocks * experts * sizeof(int) : 0;
   return GP_OK;
 }
 
