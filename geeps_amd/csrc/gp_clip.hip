@@ -114,68 +114,77 @@ __device__ __forceinline__ void square_chunk(double &sum, const Chunk &c) {
 }
 
 template <bool NT>
+__device__ __forceinline__ void square_any(double &sum, const Chunk &c) {
+  if (c.type == GP_F32)
+    square_chunk<float, NT>(sum, c);
+  else if (c.type == GP_BF16)
+    square_chunk<__bf16, NT>(sum, c);
+  else
+    square_chunk<_Float16, NT>(sum, c);
+}
+
+// The first `past` chunks go past the caches (non-temporal), the others are left
+// there for the second pass.
 __global__ __launch_bounds__(kClipBlock) void grad_square_kernel(const Chunk *__restrict__ chunks, unsigned count,
-                                                                 double *__restrict__ partial) {
+                                                                 unsigned past, double *__restrict__ partial) {
   double sum = 0.0;
   Chunk next = {};
   if (blockIdx.x < count) next = chunks[blockIdx.x];
   for (unsigned k = blockIdx.x; k < count; k += gridDim.x) {
     const Chunk c = next;
     if (k + gridDim.x < count) next = chunks[k + gridDim.x];  // asked for before this chunk's values are
-    if (c.type == GP_F32)
-      square_chunk<float, NT>(sum, c);
-    else if (c.type == GP_BF16)
-      square_chunk<__bf16, NT>(sum, c);
+    if (k < past)
+      square_any<true>(sum, c);
     else
-      square_chunk<_Float16, NT>(sum, c);
+      square_any<false>(sum, c);
   }
   sum = block_sum(sum);
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
-// O: the gradient's own type, or float; one rounding.
-template <typename E, typename O>
-__device__ __forceinline__ void store_scaled(O *out, typename Vec<E>::F v) {
-  if constexpr (sizeof(O) == sizeof(E)) {
-    store_raw(out, from_float<O>(v));
-  } else {
-#pragma unroll
-    for (int h = 0; h < Vec<E>::N / 4; ++h) {
-      Vec<float>::F q = {v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
-      store_raw(out + 4 * h, q);
-    }
-  }
-}
+// N values next to each other, wherever they start.
+template <typename E, int N>
+struct Group {
+  typedef E Raw __attribute__((ext_vector_type(N)));
+  typedef Raw Loose __attribute__((aligned(sizeof(E))));
+  typedef float F __attribute__((ext_vector_type(N)));
+};
 
+// O: the gradient's own type, or float; one rounding.  Past the caches (61 M bf16
+// 60 us, 74 through them; 61 M floats 116, not 144), whose lines the stores must
+// then fill whole: a lane takes the values of 16 bytes of the output, next to its
+// neighbours' (bf16 to float 77 us; 119 in 16-byte loads with two stores 32 bytes
+// apart).  Rows that start off a 16-byte boundary gain less: 122 us, not 144.
 template <typename E, typename O>
 __device__ __forceinline__ void scale_chunk(const Chunk &c, const Factor &f) {
-  using V = Vec<E>;
-  constexpr int U = 4;
-  constexpr unsigned kStep = kClipBlock * V::N;
+  constexpr int N = 16 / (int)sizeof(O);
+  constexpr int U = 4 * (int)(sizeof(O) / sizeof(E));  // 64 bytes of a lane's loads in flight
+  using G = Group<E, N>;
+  using H = Group<O, N>;
+  constexpr unsigned kStep = kClipBlock * N;
   const E *in = static_cast<const E *>(c.in);
   O *out = static_cast<O *>(c.out);
-  unsigned i = threadIdx.x * V::N;
-  for (; i + (U - 1) * kStep + V::N <= c.n; i += U * kStep) {
-    typename V::Raw v[U];
+  auto load = [&](unsigned i) {
+    return __builtin_nontemporal_load(reinterpret_cast<const typename G::Loose *>(in + i));
+  };
+  auto store = [&](unsigned i, typename G::Raw v) {
+    const typename G::F s = f.skip ? (typename G::F)(0.0f) : f.f * __builtin_convertvector(v, typename G::F);
+    __builtin_nontemporal_store(__builtin_convertvector(s, typename H::Raw),
+                                reinterpret_cast<typename H::Loose *>(out + i));
+  };
+  unsigned i = threadIdx.x * N;
+  for (; i + (U - 1) * kStep + N <= c.n; i += U * kStep) {
+    typename G::Raw v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = load_raw(in + i + u * kStep);
+    for (int u = 0; u < U; ++u) v[u] = load(i + u * kStep);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const typename V::F s = f.skip ? (typename V::F)(0.0f) : f.f * to_float<E>(v[u]);
-      store_scaled<E, O>(out + i + u * kStep, s);
-    }
+    for (int u = 0; u < U; ++u) store(i + u * kStep, v[u]);
   }
-  for (; i < c.n; i += kStep) {
-    const unsigned left = c.n - i;
-    const typename V::F v = to_float<E>(left >= (unsigned)V::N ? load_raw(in + i) : load_part(in + i, left));
-    const typename V::F s = f.skip ? (typename V::F)(0.0f) : f.f * v;
-    if (left >= (unsigned)V::N) {
-      store_scaled<E, O>(out + i, s);
-    } else {
+  for (; i + N <= c.n; i += kStep) store(i, load(i));
+  if (i < c.n) {
 #pragma unroll
-      for (int j = 0; j < V::N; ++j)
-        if (j < (int)left) out[i + j] = (O)s[j];
-    }
+    for (int j = 0; j < N; ++j)
+      if (i + j < c.n) out[i + j] = (O)(f.skip ? 0.0f : f.f * (float)in[i + j]);
   }
 }
 
@@ -404,18 +413,20 @@ struct gp_grad_plan_s {
 
 namespace {
 
-// Gradients that the caches may hold until the second pass are read through
-// them (75 MB of bf16: both passes 38.0 us, 40.3 past them), larger lists past
-// them (1.2 GB: the first pass 180 us, 212 through them).
-constexpr size_t kCachedBytes = (size_t)192 << 20;
+// What the memory-side cache holds of the gradients until the second pass, which
+// starts where the first ended.  1.2 GB of bf16, both passes: 603 us; 2 % more
+// with 192 or 384 MiB left there, 6 % with none, 8 % with all of it read through
+// the caches.
+constexpr size_t kCachedBytes = (size_t)256 << 20;
+
+unsigned chunks_past(const gp_grad_plan_s *p) {
+  if (p->bytes <= kCachedBytes) return 0;
+  return (unsigned)((double)p->count * ((double)(p->bytes - kCachedBytes) / (double)p->bytes));
+}
 
 void launch_grad_square(const gp_grad_plan_s *p, unsigned grid, double *partial, hipStream_t s) {
-  if (p->bytes <= kCachedBytes)
-    hipLaunchKernelGGL((grad_square_kernel<false>), dim3(grid), dim3(kClipBlock), 0, s, (const Chunk *)p->chunks,
-                       (unsigned)p->count, partial);
-  else
-    hipLaunchKernelGGL((grad_square_kernel<true>), dim3(grid), dim3(kClipBlock), 0, s, (const Chunk *)p->chunks,
-                       (unsigned)p->count, partial);
+  hipLaunchKernelGGL(grad_square_kernel, dim3(grid), dim3(kClipBlock), 0, s, (const Chunk *)p->chunks,
+                     (unsigned)p->count, chunks_past(p), partial);
 }
 
 int check_grad_plan(const gp_grad_plan_s *p, const void *workspace) {
