@@ -7,6 +7,8 @@
 //
 // The moves are bound by HBM: no row takes part in a product with another.
 
+#include <type_traits>
+
 #include "gp_device.hpp"
 
 namespace {
@@ -61,12 +63,14 @@ struct SortShared {
 };
 
 // After it, s.run holds every wave's first places and s.total / s.offset the
-// groups.  lo: the block's first choice; hist: NULL to count all n.  `key` is the lane's own first choice, so that a wave with one step
-// reads its ids once.
+// groups.  lo: the block's first choice, from..to: the wave's, all: they are all
+// there are.  hist: the counts of `parts` runs of `per` choices, or NULL to
+// count all n.  `key` is the lane's own first choice, so that a wave with one
+// step reads its ids once.
 template <int W, typename I>
 __device__ __forceinline__ void route_prepare(SortShared<W> &s, int key, const I *__restrict__ ids, unsigned n,
-                                              unsigned lo, unsigned from, unsigned to, int experts, int align,
-                                              const int *__restrict__ hist, unsigned block, unsigned blocks) {
+                                              unsigned lo, unsigned from, unsigned to, bool all, int experts,
+                                              int align, const int *__restrict__ hist, unsigned per, unsigned parts) {
   constexpr int kThreads = W * kWave;
   constexpr int kPer = kMaxExperts / kThreads;  // experts to a thread, next to each other
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
@@ -82,25 +86,32 @@ __device__ __forceinline__ void route_prepare(SortShared<W> &s, int key, const I
     const int k = key_of(ids[i], experts);
     if (k < experts) atomicAdd(&s.run[wave][k], 1);
   }
-  if (blocks > 1 && !hist) {
+  if (!all && !hist) {
     for (unsigned i = tid; i < n; i += kThreads) {
       const int k = key_of(ids[i], experts);
       if (k >= experts) continue;
       atomicAdd(i < lo ? &s.before[k] : &s.total[k], 1);
     }
-  } else if (blocks > 1) {
-    const int parts = kThreads / experts;  // thread (part, expert) sums every parts-th block's count
-    const int e = tid % experts, part = tid / experts;
-    if (part < parts) {
+  } else if (!all) {
+    const unsigned mine = lo / per;            // the run that holds lo: its choices before lo one by one
+    const unsigned rows = kThreads / experts;  // thread (row, expert) sums every rows-th run's count
+    const unsigned e = tid % experts, row = tid / experts;
+    if (row < rows) {
       int rest = 0, before = 0;
 #pragma unroll 8
-      for (unsigned g = part; g < blocks; g += parts) {
+      for (unsigned g = row; g < parts; g += rows) {
         const int c = hist[(size_t)g * experts + e];
-        rest += g < block ? 0 : c;
-        before += g < block ? c : 0;
+        rest += g < mine ? 0 : c;
+        before += g < mine ? c : 0;
       }
       atomicAdd(&s.total[e], rest);
       atomicAdd(&s.before[e], before);
+    }
+    for (unsigned i = mine * per + tid; i < lo; i += kThreads) {
+      const int k = key_of(ids[i], experts);
+      if (k >= experts) continue;
+      atomicAdd(&s.before[k], 1);
+      atomicSub(&s.total[k], 1);
     }
   }
   __syncthreads();
@@ -110,7 +121,7 @@ __device__ __forceinline__ void route_prepare(SortShared<W> &s, int key, const I
     const int e = tid * kPer + j;
     int mine = 0;
     if (e < experts) {
-      if (blocks == 1) {
+      if (all) {
 #pragma unroll
         for (int w = 0; w < W; ++w) mine += s.run[w][e];
       } else {
@@ -177,7 +188,7 @@ __global__ __launch_bounds__(kSortBlock) void route_place_kernel(
   const unsigned per_wave = per_block / kSortWaves;
   const unsigned from = min(hi, lo + wave * per_wave), to = min(hi, from + per_wave);
   int key = from + lane < to ? key_of(ids[from + lane], experts) : experts;
-  route_prepare(s, key, ids, n, lo, from, to, experts, align, hist, blockIdx.x, gridDim.x);
+  route_prepare(s, key, ids, n, lo, from, to, gridDim.x == 1, experts, align, hist, per_block, gridDim.x);
   if (blockIdx.x == 0) {
     if (tid < experts) {
       counts[tid] = s.total[tid];
@@ -210,18 +221,26 @@ constexpr int kMoveWaves = kMoveBlock / kWave;
 constexpr unsigned kZeroRows = 16;  // places that one wave looks through for rows to clear
 
 // Rows are read and written once, so they go past the caches (non-temporal):
-// 16384 tokens of 4096 bf16, 8 choices: dispatch 209 us, not 242, combine 207,
-// not 240, its gradient 415, not 457.  But not the loads of rows that start off
-// a 16-byte boundary, whose lines two of a wave's accesses share: the gradient
-// of 4099 tokens of 1001 floats took 27 us with them, 22 without.
+// 8192 tokens of 4096 bf16, 8 choices: dispatch 109 us, 125 through them, combine
+// 103, 111 with its loads through them.  But
+//  - loads and dispatch's stores of rows that start off a 16-byte boundary go
+//    through them: two of a wave's accesses share a line there (32768 tokens of
+//    1001 fp16, 10 choices: dispatch 203 us, 237 past the caches);
+//  - combine_grad's stores do, where all of its rows fit the memory-side cache
+//    (8192 tokens of 2048 bf16, 8 choices: 90 us, 103 past it; 12000 tokens: 152,
+//    149 past it), and combine's, where the rows do not fit and leave it to y
+//    (16384 tokens of 4096 bf16: 205 us, 212 past it; 8192 of 2048: 52, 52).
+constexpr size_t kCachedRows = (size_t)256 << 20;
+
 struct Shape {
   unsigned tokens, k, rows, width;
   unsigned splits;       // waves that share a token's columns
   unsigned token_waves;  // tokens * splits
+  unsigned first_block;  // of this launch
 };
 
 // Clears row first + lane for every lane that finds it `empty`.
-template <typename E>
+template <typename E, bool NT>
 __device__ __forceinline__ void clear_rows(E *__restrict__ out, size_t stride, unsigned first, bool empty,
                                            unsigned width) {
   using V = Vec<E>;
@@ -231,28 +250,35 @@ __device__ __forceinline__ void clear_rows(E *__restrict__ out, size_t stride, u
     for (unsigned c = lane * V::N; c < width; c += kWave * V::N) {
       const typename V::Raw zero = (E)0.0f;
       if (c + V::N <= width)
-        store_raw<E, true>(row + c, zero);
+        store_raw<E, NT>(row + c, zero);
       else
         store_part(row + c, zero, width - c);
     }
   }
 }
 
-// A token's columns of one wave, to the row of every choice; p: lane c's row.
-template <typename E>
+// A row's 16 bytes from column c on.
+template <typename E, bool NT = false>
+__device__ __forceinline__ typename Vec<E>::Raw load_at(const E *__restrict__ row, unsigned c, unsigned width) {
+  return c + Vec<E>::N <= width ? load_raw<E, NT>(row + c) : load_part(row + c, (int)(width - c));
+}
+
+// A token's columns of one wave, to the row of every choice; p: lane c's row, v:
+// the lane's first values (any, where its column is behind the row).
+template <typename E, bool NT>
 __device__ __forceinline__ void dispatch_token(E *__restrict__ out, size_t out_stride, const E *__restrict__ from,
-                                               int p, unsigned split, const Shape &d) {
+                                               int p, unsigned split, const Shape &d, typename Vec<E>::Raw v) {
   using V = Vec<E>;
   const int lane = threadIdx.x % kWave;
   const uint64_t held = __ballot((unsigned)p < d.rows);
-  for (unsigned c = (split * kWave + lane) * V::N; c < d.width; c += d.splits * kWave * V::N) {
-    const bool whole = c + V::N <= d.width;
-    const typename V::Raw v = whole ? load_raw(from + c) : load_part(from + c, d.width - c);
+  const unsigned first = (split * kWave + lane) * V::N, step = d.splits * kWave * V::N;
+  for (unsigned c = first; c < d.width; c += step) {
+    if (c != first) v = load_at(from, c, d.width);
     for (uint64_t left = held; left; left &= left - 1) {
       const int to = __builtin_amdgcn_readlane(p, __ffsll((long long)left) - 1);
       E *row = out + (size_t)to * out_stride + c;
-      if (whole)
-        store_raw<E, true>(row, v);
+      if (c + V::N <= d.width)
+        store_raw<E, NT>(row, v);
       else
         store_part(row, v, d.width - c);
     }
@@ -260,22 +286,46 @@ __device__ __forceinline__ void dispatch_token(E *__restrict__ out, size_t out_s
 }
 
 template <typename E>
+__device__ __forceinline__ typename Vec<E>::Raw first_values(const E *__restrict__ from, unsigned split,
+                                                             const Shape &d) {
+  const unsigned c = (split * kWave + threadIdx.x % kWave) * Vec<E>::N;
+  return c < d.width ? load_at(from, c, d.width) : (typename Vec<E>::Raw)((E)0.0f);
+}
+
+template <typename E, bool NT>
 __global__ __launch_bounds__(kMoveBlock) void route_dispatch_kernel(E *__restrict__ out, size_t out_stride,
                                                                     const E *__restrict__ x, size_t x_stride,
                                                                     const int *__restrict__ position,
                                                                     const int *__restrict__ order, Shape d) {
-  const unsigned wave = blockIdx.x * kMoveWaves + threadIdx.x / kWave;
+  const unsigned wave = (d.first_block + blockIdx.x) * kMoveWaves + threadIdx.x / kWave;
   const int lane = threadIdx.x % kWave;
   if (wave >= d.token_waves) {
     const unsigned first = (wave - d.token_waves) * kZeroRows, at = first + lane;
     const bool mine = lane < (int)kZeroRows && at < d.rows;
     const int o = mine ? order[at] : 0;
-    clear_rows(out, out_stride, first, mine && (o < 0 || (unsigned)o >= d.tokens * d.k), d.width);
+    clear_rows<E, NT>(out, out_stride, first, mine && (o < 0 || (unsigned)o >= d.tokens * d.k), d.width);
     return;
   }
   const unsigned t = wave / d.splits;
   const int p = lane < (int)d.k ? position[(size_t)t * d.k + lane] : -1;
-  dispatch_token(out, out_stride, x + (size_t)t * x_stride, p, wave % d.splits, d);
+  const unsigned split = wave % d.splits;
+  const E *from = x + (size_t)t * x_stride;
+  dispatch_token<E, NT>(out, out_stride, from, p, split, d, first_values(from, split, d));
+}
+
+// A row's group is the last that starts at or before it; behind the group's
+// choices the row is empty.
+template <int W>
+__device__ __forceinline__ bool row_empty(const SortShared<W> &s, int r, int experts) {
+  int lo = 0, hi = experts;  // offset[lo] <= r < offset[hi], or r is behind the last group
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (s.offset[mid] <= r)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return r - s.offset[lo] >= s.total[lo];
 }
 
 // Few choices: every block makes the places for itself, in LDS, and moves its
@@ -283,7 +333,7 @@ __global__ __launch_bounds__(kMoveBlock) void route_dispatch_kernel(E *__restric
 // calls.  16 tokens of 4096 bf16, 4 choices: see the host side.
 constexpr unsigned kSmallRoute = 1024;
 
-template <typename E, typename I>
+template <typename E, typename I, bool NT>
 __global__ __launch_bounds__(kMoveBlock) void route_sort_dispatch_kernel(
     E *__restrict__ out, size_t out_stride, const E *__restrict__ x, size_t x_stride, const I *__restrict__ ids,
     int experts, int bits, int align, int *__restrict__ position, int *__restrict__ order, int *__restrict__ counts,
@@ -291,55 +341,112 @@ __global__ __launch_bounds__(kMoveBlock) void route_sort_dispatch_kernel(
   __shared__ SortShared<kMoveWaves> s;
   __shared__ int place[kSmallRoute];
   const unsigned n = d.tokens * d.k;
+  const bool leaves = d.first_block + blockIdx.x == 0;
   const int tid = threadIdx.x, in_block = tid / kWave, lane = tid % kWave;
   const unsigned per_wave = (n + kMoveBlock - 1) / kMoveBlock * kWave;
   const unsigned from = min(n, in_block * per_wave), to = min(n, from + per_wave);
   int key = from + lane < to ? key_of(ids[from + lane], experts) : experts;
-  route_prepare(s, key, ids, n, 0u, from, to, experts, align, (const int *)nullptr, 0u, 1u);
+  route_prepare(s, key, ids, n, 0u, from, to, true, experts, align, (const int *)nullptr, 1u, 1u);
   for (unsigned i0 = from; i0 < to; i0 += kWave) {
     const unsigned i = i0 + lane;
     if (i0 != from) key = i < to ? key_of(ids[i], experts) : experts;
     const int at = route_step(s, key, experts, bits);
     if (i < to) {
       place[i] = at;
-      if (blockIdx.x == 0) {
+      if (leaves) {
         position[i] = at;
         if (at >= 0) order[at] = (int)i;
       }
     }
   }
   __syncthreads();
-  if (blockIdx.x == 0) {
+  if (leaves) {
     for (int e = tid; e < experts; e += kMoveBlock) {
       counts[e] = s.total[e];
       offsets[e] = s.offset[e];
     }
     if (tid == 0) offsets[experts] = s.offset[experts];
   }
-  const unsigned wave = blockIdx.x * kMoveWaves + in_block;
+  const unsigned wave = (d.first_block + blockIdx.x) * kMoveWaves + in_block;
   if (wave >= d.token_waves) {
-    // a row's group is the last that starts at or before it; behind the
-    // group's choices the row is empty
     const unsigned first = (wave - d.token_waves) * kZeroRows, r = first + lane;
-    bool empty = false;
-    if (lane < (int)kZeroRows && r < d.rows) {
-      int lo = 0, hi = experts;  // offset[lo] <= r < offset[hi], or r is behind the last group
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (s.offset[mid] <= (int)r)
-          lo = mid;
-        else
-          hi = mid;
-      }
-      empty = (int)r - s.offset[lo] >= s.total[lo];
-      if (empty) order[r] = -1;
-    }
-    clear_rows(out, out_stride, first, empty, d.width);
+    const bool empty = lane < (int)kZeroRows && r < d.rows && row_empty(s, (int)r, experts);
+    if (empty) order[r] = -1;
+    clear_rows<E, NT>(out, out_stride, first, empty, d.width);
     return;
   }
   const unsigned t = wave / d.splits;
   const int p = lane < (int)d.k ? place[t * d.k + lane] : -1;
-  dispatch_token(out, out_stride, x + (size_t)t * x_stride, p, wave % d.splits, d);
+  const unsigned split = wave % d.splits;
+  const E *row = x + (size_t)t * x_stride;
+  dispatch_token<E, NT>(out, out_stride, row, p, split, d, first_values(row, split, d));
+}
+
+// More choices: a block makes the places of its own share of the tokens and
+// moves them, two blocks to a CU, so the places cost no launch and no pass over
+// them of their own.  4099 tokens of 1001 floats, 3 choices: see the host side.
+template <typename E, typename I>
+__global__ __launch_bounds__(kSortBlock) void route_place_dispatch_kernel(
+    E *__restrict__ out, size_t out_stride, const E *__restrict__ x, size_t x_stride, const I *__restrict__ ids,
+    int experts, int bits, int align, const int *__restrict__ hist, unsigned per_hist, unsigned hist_parts,
+    int *position, int *__restrict__ order, int *__restrict__ counts, int *__restrict__ offsets, Shape d) {
+  __shared__ SortShared<kSortWaves> s;
+  const unsigned n = d.tokens * d.k;
+  const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
+  const unsigned first = (unsigned)((uint64_t)d.tokens * blockIdx.x / gridDim.x);
+  const unsigned last = (unsigned)((uint64_t)d.tokens * (blockIdx.x + 1) / gridDim.x);
+  const unsigned lo = first * d.k, hi = last * d.k;
+  const unsigned per_wave = (hi - lo + kSortBlock - 1) / kSortBlock * kWave;
+  const unsigned from = min(hi, lo + wave * per_wave), to = min(hi, from + per_wave);
+  int key = from + lane < to ? key_of(ids[from + lane], experts) : experts;
+  route_prepare(s, key, ids, n, lo, from, to, gridDim.x == 1, experts, align, hist, per_hist, hist_parts);
+  for (unsigned i0 = from; i0 < to; i0 += kWave) {
+    const unsigned i = i0 + lane;
+    if (i0 != from) key = i < to ? key_of(ids[i], experts) : experts;
+    const int at = route_step(s, key, experts, bits);
+    if (i < to) position[i] = at;
+    if (at >= 0) order[at] = (int)i;
+  }
+  if (blockIdx.x == 0) {
+    if (tid < experts) {
+      counts[tid] = s.total[tid];
+      offsets[tid] = s.offset[tid];
+    }
+    if (tid == 0) offsets[experts] = s.offset[experts];
+  }
+  __syncthreads();  // the block's positions are there
+  // a unit, one split of a token: the next one's row is asked for before this one's is stored
+  const unsigned units = (last - first) * d.splits;
+  auto row_of = [&](unsigned u) { return x + (size_t)(first + u / d.splits) * x_stride; };
+  auto places_of = [&](unsigned u) {
+    return lane < (int)d.k ? position[(size_t)(first + u / d.splits) * d.k + lane] : -1;
+  };
+  int p = -1;
+  typename Vec<E>::Raw v = (E)0.0f;
+  if ((unsigned)wave < units) {
+    p = places_of(wave);
+    v = first_values(row_of(wave), wave % d.splits, d);
+  }
+  for (unsigned u = wave; u < units; u += kSortWaves) {
+    const unsigned next = u + kSortWaves;
+    int next_p = -1;
+    typename Vec<E>::Raw next_v = v;
+    if (next < units) {
+      next_p = places_of(next);
+      next_v = first_values(row_of(next), next % d.splits, d);
+    }
+    dispatch_token<E, false>(out, out_stride, row_of(u), p, u % d.splits, d, v);
+    p = next_p;
+    v = next_v;
+  }
+  // rows that hold no choice: kPer of them to a wave at a time
+  constexpr unsigned kPer = 4;
+  for (unsigned r0 = (blockIdx.x * kSortWaves + wave) * kPer; r0 < d.rows; r0 += gridDim.x * kSortWaves * kPer) {
+    const unsigned r = r0 + lane;
+    const bool empty = lane < (int)kPer && r < d.rows && row_empty(s, (int)r, experts);
+    if (empty) order[r] = -1;
+    clear_rows<E, false>(out, out_stride, r0, empty, d.width);
+  }
 }
 
 // Weights: none (1), float, or the rows' own type.
@@ -372,14 +479,14 @@ __device__ __forceinline__ void combine_group(typename Vec<E>::F &acc, uint64_t 
   for (int g = 0; g < G; ++g) acc += f[g] * to_float<E>(v[g]);  // choices in order, in 32 bits
 }
 
-template <typename E, bool NT>
+template <typename E, bool NT, bool NT_OUT>
 __global__ __launch_bounds__(kMoveBlock) void route_combine_kernel(E *__restrict__ y, size_t y_stride,
                                                                    const E *__restrict__ rows, size_t row_stride,
                                                                    const int *__restrict__ position,
                                                                    const void *__restrict__ weights, int weight_type,
                                                                    Shape d) {
   using V = Vec<E>;
-  const unsigned wave = blockIdx.x * kMoveWaves + threadIdx.x / kWave;
+  const unsigned wave = (d.first_block + blockIdx.x) * kMoveWaves + threadIdx.x / kWave;
   const int lane = threadIdx.x % kWave;
   if (wave >= d.token_waves) return;
   const unsigned t = wave / d.splits, split = wave % d.splits;
@@ -398,7 +505,7 @@ __global__ __launch_bounds__(kMoveBlock) void route_combine_kernel(E *__restrict
     if (n >= 2) combine_group<E, 2, NT>(acc, left, rows, row_stride, p, w, c, whole, d.width), n -= 2;
     if (n >= 1) combine_group<E, 1, NT>(acc, left, rows, row_stride, p, w, c, whole, d.width);
     if (whole)
-      store_raw<E, true>(to + c, from_float<E>(acc));
+      store_raw<E, NT_OUT>(to + c, from_float<E>(acc));
     else
       store_part(to + c, from_float<E>(acc), d.width - c);
   }
@@ -410,7 +517,7 @@ __global__ __launch_bounds__(kMoveBlock) void route_combine_kernel(E *__restrict
 // are 32-bit sums, lane by lane, then over the wave, then over the splits' waves
 // in their order.
 // ---------------------------------------------------------------------------
-template <typename E, int G, bool NT>
+template <typename E, int G, bool NT, bool NT_OUT>
 __device__ __forceinline__ void grad_group(uint64_t &left, E *__restrict__ d_rows, size_t d_stride,
                                            const E *__restrict__ dy, const E *__restrict__ rows, size_t row_stride,
                                            int p, float w, unsigned first, unsigned step, unsigned width, float &dot) {
@@ -445,7 +552,7 @@ __device__ __forceinline__ void grad_group(uint64_t &left, E *__restrict__ d_row
       E *row = d_rows + at[g] * d_stride + c;
       const typename V::Raw out = from_float<E>(f[g] * o);
       if (whole)
-        store_raw<E, true>(row, out);
+        store_raw<E, NT_OUT>(row, out);
       else
         store_part(row, out, part);
     }
@@ -458,7 +565,7 @@ __device__ __forceinline__ void grad_group(uint64_t &left, E *__restrict__ d_row
 }
 
 // S waves share a token (d.splits = S); a block holds kMoveWaves / S tokens.
-template <typename E, int S, bool NT>
+template <typename E, int S, bool NT, bool NT_OUT>
 __global__ __launch_bounds__(kMoveBlock) void route_combine_grad_kernel(
     E *__restrict__ d_rows, size_t d_stride, void *__restrict__ d_weights, const E *__restrict__ dy, size_t dy_stride,
     const E *__restrict__ rows, size_t row_stride, const int *__restrict__ position, const int *__restrict__ order,
@@ -466,14 +573,14 @@ __global__ __launch_bounds__(kMoveBlock) void route_combine_grad_kernel(
   using V = Vec<E>;
   __shared__ float part[kMoveWaves][kWave];
   const unsigned in_block = threadIdx.x / kWave;
-  const unsigned wave = blockIdx.x * kMoveWaves + in_block;
+  const unsigned wave = (d.first_block + blockIdx.x) * kMoveWaves + in_block;
   const int lane = threadIdx.x % kWave;
   const bool moves = wave < d.token_waves;
   if (!moves) {  // these waves clear, and meet the others at the barrier below
     const unsigned first = (wave - d.token_waves) * kZeroRows, at = first + lane;
     const bool look = lane < (int)kZeroRows && at < d.rows;
     const int o = look ? order[at] : 0;
-    clear_rows(d_rows, d_stride, first, look && (o < 0 || (unsigned)o >= d.tokens * d.k), d.width);
+    clear_rows<E, NT_OUT>(d_rows, d_stride, first, look && (o < 0 || (unsigned)o >= d.tokens * d.k), d.width);
   }
   const unsigned t = wave / S, split = wave % S;
   const size_t a = (size_t)t * d.k + lane;
@@ -487,10 +594,10 @@ __global__ __launch_bounds__(kMoveBlock) void route_combine_grad_kernel(
     const unsigned first = (split * kWave + lane) * V::N, step = S * kWave * V::N;
     uint64_t left = held;
     int n = __popcll(held);
-    for (; n >= 8; n -= 8) grad_group<E, 8, NT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot);
-    if (n >= 4) grad_group<E, 4, NT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot), n -= 4;
-    if (n >= 2) grad_group<E, 2, NT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot), n -= 2;
-    if (n >= 1) grad_group<E, 1, NT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot);
+    for (; n >= 8; n -= 8) grad_group<E, 8, NT, NT_OUT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot);
+    if (n >= 4) grad_group<E, 4, NT, NT_OUT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot), n -= 4;
+    if (n >= 2) grad_group<E, 2, NT, NT_OUT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot), n -= 2;
+    if (n >= 1) grad_group<E, 1, NT, NT_OUT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot);
   }
   if constexpr (S > 1) {
     part[in_block][lane] = dot;
@@ -515,12 +622,25 @@ __global__ __launch_bounds__(kMoveBlock) void route_combine_grad_kernel(
 // Up to this many choices every block counts them all for itself: one launch
 // (4.6 us at 4096 choices, 5.5 at 8192, 7.2 at 16384, against 6.3, 6.7 and 7.3
 // of two launches, the second of which costs the caller 3 more).
-constexpr size_t kSelfCounted = 16384;
+constexpr size_t kSelfCounted = GP_ROUTE_UNCOUNTED;
 // Above, b blocks cost about 1.2 us for each of their n / (1024 b) steps and
 // 2.6e-4 us for each of the b * experts counts that every block sums: least at
 // b * b = 4.4 n / experts.  131072 choices of 512 experts: 25.5 us at 128
 // blocks, 18.0 at 64, 16.1 at 32; of 128: 11.5, 10.3, 11.3.
 constexpr size_t kMostSortBlocks = 1024;
+
+// Up to this many bytes of tokens and of rows for them, the blocks that make the
+// places also move the tokens: the launch that it saves is worth more than the
+// blocks' fixed shares of the tokens cost.  In one launch (more than 16384
+// choices: two), and in one more:
+//   4099 tokens of 1001 floats, 3 choices (66 MB)   21.9 us, 27.4
+//   700 of 7168 bf16, 6 choices (70 MB)             26.8 us, 33.7
+//   2000 of 2048 bf16, 8 choices (74 MB)            38.0 us, 50.3
+//   4000 of 2048 bf16, 4 choices (82 MB)            22.4 us, 23.7
+//   6000 of 2048 bf16, 4 choices (123 MB)           26.8 us, 27.5
+//   10000 of 4000 bf16, 1 choice (160 MB)           39.0 us, 32.3
+//   8192 of 2048 bf16, 6 choices (235 MB)           53.6 us, 46.0
+constexpr size_t kPlaceAndMove = (size_t)96 << 20;
 
 struct SortPlan {
   unsigned blocks, per_block;
@@ -567,16 +687,19 @@ int check_move(size_t tokens, size_t k, size_t rows, size_t width, int type) {
   return GP_OK;
 }
 
-// Waves over a token's columns.  Eight, where there are as many steps of 64
-// lanes, keep a row's accesses together in time (8192 tokens of 2048 bf16, 8
-// choices: dispatch 52 us, 64 with 2 waves); more when tokens are few, until
-// the chip has 4 waves per SIMD.
-unsigned pick_splits(size_t tokens, size_t width, int type) {
+// Waves over a token's columns: `least`, where there are as many steps of 64
+// lanes, more when tokens are few, until the chip has 4 waves per SIMD.  They
+// keep a row's accesses together in time (8192 tokens of 2048 bf16, 8 choices:
+// dispatch 52 us, 64 with 2 waves).  Eight for combine, and for dispatch with up
+// to three choices (30000 tokens of 2048 floats, 3 choices: 175 us, 178 with
+// four; 1 choice of 4000 bf16: 91, 95); with more choices four (20000 of 7168
+// bf16, 4 choices: 268 us, 289 with eight; 16384 of 4096, 8 choices: 245, 253).
+unsigned pick_splits(size_t tokens, size_t width, int type, size_t least) {
   const size_t per_step = kWave * 16 / type_size(type);
   const size_t steps = (width + per_step - 1) / per_step;
   const size_t want = (size_t)device_cus() * 16;
   size_t s = tokens ? want / tokens : 1;
-  if (s < 8) s = 8;
+  if (s < least) s = least;
   return (unsigned)(s < steps ? s : (steps ? steps : 1));
 }
 
@@ -584,11 +707,21 @@ bool rows_aligned(const void *p, size_t stride, int type) {
   return ((reinterpret_cast<uintptr_t>(p) | stride * type_size(type)) & 15) == 0;
 }
 
-int check_grid(size_t waves, unsigned *blocks) {
-  const size_t b = (waves + kMoveWaves - 1) / kMoveWaves;
-  GP_REQUIRE(b <= (size_t)INT32_MAX, "too many rows for one launch");
-  *blocks = (unsigned)b;
+int check_grid(size_t waves, size_t *blocks) {
+  GP_REQUIRE(waves <= UINT32_MAX, "too many rows for one call");
+  *blocks = (waves + kMoveWaves - 1) / kMoveWaves;
   return GP_OK;
+}
+
+// A grid has at most 2^32 threads: longer ones go in several launches.
+constexpr size_t kMostBlocks = (size_t)1 << 23;
+
+template <typename F>
+void launch_moves(size_t blocks, Shape d, F launch) {
+  for (size_t b = 0; b < blocks; b += kMostBlocks) {
+    d.first_block = (unsigned)b;
+    launch(dim3((unsigned)(blocks - b < kMostBlocks ? blocks - b : kMostBlocks)), d);
+  }
 }
 
 #define GP_TRY(expr)             \
@@ -624,14 +757,14 @@ size_t strided_bytes(size_t rows, size_t stride, size_t width, int type) {
 }
 
 int plan_dispatch(const void *out, size_t out_stride, const void *x, size_t x_stride, int type, size_t tokens,
-                  size_t k, size_t rows, size_t width, Shape *d, unsigned *blocks) {
+                  size_t k, size_t rows, size_t width, Shape *d, size_t *blocks) {
   GP_TRY(check_move(tokens, k, rows, width, type));
   GP_REQUIRE(out && (tokens == 0 || x), "null out or x");
   GP_REQUIRE(out_stride >= width && x_stride >= width, "row stride smaller than the width");
   GP_REQUIRE(!bytes_overlap(out, strided_bytes(rows, out_stride, width, type), x,
                             strided_bytes(tokens, x_stride, width, type)),
              "out overlaps x");
-  *d = Shape{(unsigned)tokens, (unsigned)k, (unsigned)rows, (unsigned)width, pick_splits(tokens, width, type), 0};
+  *d = Shape{(unsigned)tokens, (unsigned)k, (unsigned)rows, (unsigned)width, pick_splits(tokens, width, type, k < 4 ? 8 : 4), 0, 0};
   const size_t waves = tokens * (size_t)d->splits;
   GP_TRY(check_grid(waves + (rows + kZeroRows - 1) / kZeroRows, blocks));
   d->token_waves = (unsigned)waves;
@@ -689,12 +822,20 @@ int gp_route_dispatch(void *out, size_t out_stride, const void *x, size_t x_stri
   if (rows == 0 || width == 0) return GP_OK;
   GP_REQUIRE(order && (tokens == 0 || position), "null position or order");
   Shape d;
-  unsigned blocks = 0;
+  size_t blocks = 0;
   GP_TRY(plan_dispatch(out, out_stride, x, x_stride, type, tokens, k, rows, width, &d, &blocks));
   with_type(type, [&](auto e) {
     using E = decltype(e);
-    hipLaunchKernelGGL((route_dispatch_kernel<E>), dim3(blocks), dim3(kMoveBlock), 0, (hipStream_t)s,
-                       static_cast<E *>(out), out_stride, static_cast<const E *>(x), x_stride, position, order, d);
+    auto go = [&](auto kernel) {
+      launch_moves(blocks, d, [&](dim3 grid, Shape d) {
+        hipLaunchKernelGGL(kernel, grid, dim3(kMoveBlock), 0, (hipStream_t)s, static_cast<E *>(out), out_stride,
+                           static_cast<const E *>(x), x_stride, position, order, d);
+      });
+    };
+    if (rows_aligned(out, out_stride, type))
+      go(route_dispatch_kernel<E, true>);
+    else
+      go(route_dispatch_kernel<E, false>);
   });
   GP_HIP_TRY(hipGetLastError());
   return GP_OK;
@@ -706,7 +847,7 @@ int gp_route_sort_dispatch(void *out, size_t out_stride, const void *x, size_t x
                            size_t workspace_bytes, gp_stream s) {
   GP_TRY(check_groups(tokens, k, experts, align));
   const size_t rows = grouped_rows(tokens, k, experts, align), n = tokens * k;
-  if (n == 0 || n > kSmallRoute || width == 0) {
+  if (n == 0 || width == 0 || (n > kSmallRoute && (n + tokens) * width * type_size(type) > kPlaceAndMove)) {
     GP_TRY(check_move(tokens, k, rows, width, type));
     GP_TRY(gp_route_sort(ids, id_bits, tokens, k, experts, align, position, order, counts, offsets, workspace,
                          workspace_bytes, s));
@@ -715,17 +856,39 @@ int gp_route_sort_dispatch(void *out, size_t out_stride, const void *x, size_t x
   GP_REQUIRE(id_bits == 32 || id_bits == 64, "ids must be 32 or 64 bits wide");
   GP_REQUIRE(ids && position && order && counts && offsets, "null ids, position, order, counts or offsets");
   Shape d;
-  unsigned blocks = 0;
+  size_t blocks = 0;
   GP_TRY(plan_dispatch(out, out_stride, x, x_stride, type, tokens, k, rows, width, &d, &blocks));
   const SortPlan p = sort_plan(n, experts);
+  int *hist = p.counted ? static_cast<int *>(workspace) : nullptr;
+  GP_REQUIRE(!p.counted || (hist && workspace_bytes >= (size_t)p.blocks * experts * sizeof(int)),
+             "workspace missing or too small");
   with_type(type, [&](auto e) {
     using E = decltype(e);
     auto go = [&](auto id) {
       using I = decltype(id);
-      hipLaunchKernelGGL((route_sort_dispatch_kernel<E, I>), dim3(blocks), dim3(kMoveBlock), 0, (hipStream_t)s,
-                         static_cast<E *>(out), out_stride, static_cast<const E *>(x), x_stride,
-                         static_cast<const I *>(ids), (int)experts, p.bits, (int)align, position, order, counts,
-                         offsets, d);
+      const I *in = static_cast<const I *>(ids);
+      if (n <= kSmallRoute) {
+        auto small = [&](auto kernel) {
+          launch_moves(blocks, d, [&](dim3 grid, Shape d) {
+            hipLaunchKernelGGL(kernel, grid, dim3(kMoveBlock), 0, (hipStream_t)s, static_cast<E *>(out), out_stride,
+                               static_cast<const E *>(x), x_stride, in, (int)experts, p.bits, (int)align, position,
+                               order, counts, offsets, d);
+          });
+        };
+        if (rows_aligned(out, out_stride, type))
+          small(route_sort_dispatch_kernel<E, I, true>);
+        else
+          small(route_sort_dispatch_kernel<E, I, false>);
+        return;
+      }
+      if (p.counted)
+        hipLaunchKernelGGL((route_count_kernel<I>), dim3(p.blocks), dim3(kSortBlock), 0, (hipStream_t)s, in,
+                           (unsigned)n, p.per_block, (int)experts, hist);
+      const size_t most = (size_t)device_cus() * 2;
+      hipLaunchKernelGGL((route_place_dispatch_kernel<E, I>), dim3((unsigned)(tokens < most ? tokens : most)),
+                         dim3(kSortBlock), 0, (hipStream_t)s, static_cast<E *>(out), out_stride,
+                         static_cast<const E *>(x), x_stride, in, (int)experts, p.bits, (int)align,
+                         (const int *)hist, p.per_block, p.blocks, position, order, counts, offsets, d);
     };
     id_bits == 64 ? go((int64_t)0) : go((int32_t)0);
   });
@@ -745,21 +908,25 @@ int gp_route_combine(void *y, size_t y_stride, const void *rows_in, size_t row_s
                             strided_bytes(rows, row_stride, width, type)),
              "y overlaps the rows");
   const int wt = !weights ? kNoWeights : weight_type == GP_F32 ? kFloatWeights : kRowWeights;
-  Shape d{(unsigned)tokens, (unsigned)k, (unsigned)rows, (unsigned)width, pick_splits(tokens, width, type), 0};
+  Shape d{(unsigned)tokens, (unsigned)k, (unsigned)rows, (unsigned)width, pick_splits(tokens, width, type, 8), 0, 0};
   const size_t waves = tokens * (size_t)d.splits;
-  unsigned blocks = 0;
+  size_t blocks = 0;
   GP_TRY(check_grid(waves, &blocks));
   d.token_waves = (unsigned)waves;
   with_type(type, [&](auto e) {
     using E = decltype(e);
     auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kMoveBlock), 0, (hipStream_t)s, static_cast<E *>(y), y_stride,
-                         static_cast<const E *>(rows_in), row_stride, position, weights, wt, d);
+      launch_moves(blocks, d, [&](dim3 grid, Shape d) {
+        hipLaunchKernelGGL(kernel, grid, dim3(kMoveBlock), 0, (hipStream_t)s, static_cast<E *>(y), y_stride,
+                           static_cast<const E *>(rows_in), row_stride, position, weights, wt, d);
+      });
     };
-    if (rows_aligned(rows_in, row_stride, type))
-      go(route_combine_kernel<E, true>);
+    if (!rows_aligned(rows_in, row_stride, type))
+      go(route_combine_kernel<E, false, true>);
+    else if (rows * width * type_size(type) > kCachedRows && rows_aligned(y, y_stride, type))
+      go(route_combine_kernel<E, true, false>);
     else
-      go(route_combine_kernel<E, false>);
+      go(route_combine_kernel<E, true, true>);
   });
   GP_HIP_TRY(hipGetLastError());
   return GP_OK;
@@ -778,7 +945,6 @@ int gp_route_combine_grad(void *d_rows, size_t d_stride, void *d_weights, const 
   GP_REQUIRE(d_stride >= width && dy_stride >= width && row_stride >= width, "row stride smaller than the width");
   const size_t db = strided_bytes(rows, d_stride, width, type), rb = strided_bytes(rows, row_stride, width, type);
   const size_t yb = strided_bytes(tokens, dy_stride, width, type);
-  // in place (the same rows and stride) every element is read before it is written, by the same lane
   GP_REQUIRE(!bytes_overlap(d_rows, db, dy, yb), "d_rows overlaps dy");
   GP_REQUIRE(!bytes_overlap(d_rows, db, rows_in, rb), "d_rows overlaps the rows");
   const int wt = weight_type == GP_F32 ? kFloatWeights : kRowWeights;
@@ -788,22 +954,33 @@ int gp_route_combine_grad(void *d_rows, size_t d_stride, void *d_weights, const 
   const bool aligned = rows_aligned(rows_in, row_stride, type);
   const size_t step = kWave * 16 / type_size(type);
   const unsigned splits = width <= step || (!aligned && width <= 4 * step && tokens >= 4096) ? 1 : 4;
-  Shape d{(unsigned)tokens, (unsigned)k, (unsigned)rows, (unsigned)width, splits, 0};
+  Shape d{(unsigned)tokens, (unsigned)k, (unsigned)rows, (unsigned)width, splits, 0, 0};
   const size_t waves = tokens * (size_t)d.splits;
-  unsigned blocks = 0;
+  size_t blocks = 0;
   GP_TRY(check_grid(waves + (rows + kZeroRows - 1) / kZeroRows, &blocks));
   d.token_waves = (unsigned)waves;
   with_type(type, [&](auto e) {
     using E = decltype(e);
     auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kMoveBlock), 0, (hipStream_t)s, static_cast<E *>(d_rows), d_stride,
-                         d_weights, static_cast<const E *>(dy), dy_stride, static_cast<const E *>(rows_in), row_stride,
-                         position, order, weights, wt, d);
+      launch_moves(blocks, d, [&](dim3 grid, Shape d) {
+        hipLaunchKernelGGL(kernel, grid, dim3(kMoveBlock), 0, (hipStream_t)s, static_cast<E *>(d_rows), d_stride,
+                           d_weights, static_cast<const E *>(dy), dy_stride, static_cast<const E *>(rows_in),
+                           row_stride, position, order, weights, wt, d);
+      });
+    };
+    auto pick = [&](auto s) {
+      constexpr int S = decltype(s)::value;
+      if (!aligned)
+        go(route_combine_grad_kernel<E, S, false, true>);
+      else if (rows * width * type_size(type) <= kCachedRows)
+        go(route_combine_grad_kernel<E, S, true, false>);
+      else
+        go(route_combine_grad_kernel<E, S, true, true>);
     };
     if (splits == 4)
-      aligned ? go(route_combine_grad_kernel<E, 4, true>) : go(route_combine_grad_kernel<E, 4, false>);
+      pick(std::integral_constant<int, 4>());
     else
-      aligned ? go(route_combine_grad_kernel<E, 1, true>) : go(route_combine_grad_kernel<E, 1, false>);
+      pick(std::integral_constant<int, 1>());
   });
   GP_HIP_TRY(hipGetLastError());
   return GP_OK;

@@ -35,6 +35,7 @@ class DoubleIndex(ctypes.Structure):
 
 GP_MAX_SEGMENTS = 64  # include/gp_reduce.h
 GP_F32, GP_BF16, GP_F16 = 0, 1, 2
+GP_ROUTE_UNCOUNTED = 16384
 GP_CLIP_WORKSPACE_BYTES = 16384
 GP_CLIP_PROPAGATE, GP_CLIP_SKIP = 0, 1
 

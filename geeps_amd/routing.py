@@ -99,28 +99,22 @@ def _rows2d(t, name, dtype=None, device=None, width=None) -> int:
     return stride
 
 
-def _index(t, name, device, shape=None) -> None:
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.int32 or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 CUDA tensor")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on another device")
-    if shape is not None and tuple(t.shape) != shape:
-        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
-
-
 def _route(route, device):
-    """(tokens, k, rows) of a route."""
-    _index(route.position, "route.position", device)
-    _index(route.order, "route.order", device)
-    if route.position.dim() != 2 or route.order.dim() != 1:
+    """(tokens, k, rows) of a route; device: a GPU's."""
+    position, order = route.position, route.order
+    for t, name in ((position, "route.position"), (order, "route.order")):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 CUDA tensor")
+        if t.device != device:
+            raise ValueError(f"{name} is on another device")
+    if position.dim() != 2 or order.dim() != 1:
         raise ValueError("route.position must have shape (tokens, k) and route.order (rows,)")
-    tokens, k = route.position.shape
-    return tokens, k, route.order.shape[0]
+    return *position.shape, order.shape[0]
 
 
 def _out(out, name, shape, like):
     if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device), shape[1]
+        return like.new_empty(shape), shape[1]
     stride = _rows2d(out, name, like.dtype, like.device, shape[1])
     if out.shape[0] < shape[0]:
         raise ValueError(f"{name} has {out.shape[0]} rows, {shape[0]} are written")
@@ -156,13 +150,15 @@ def group_rows(tokens: int, k: int, num_experts: int, align: int = 1) -> int:
 
 def _new_route(tokens, k, rows, num_experts, device):
     """The route's tensors and the sort's workspace, of one allocation."""
-    need = ctypes.c_size_t()
-    check(native.lib().gp_route_workspace(tokens, k, num_experts, ctypes.byref(need)), "gp_route_workspace")
-    sizes = (tokens * k, rows, num_experts, num_experts + 1)
-    if need.value:
-        sizes += (need.value // 4,)
+    sizes, size = [tokens * k, rows, num_experts, num_experts + 1], 0
+    if sizes[0] > native.GP_ROUTE_UNCOUNTED:
+        need = ctypes.c_size_t()
+        check(native.lib().gp_route_workspace(tokens, k, num_experts, ctypes.byref(need)), "gp_route_workspace")
+        size = need.value
+        sizes.append(size // 4)
     parts = torch.empty(sum(sizes), dtype=torch.int32, device=device).split_with_sizes(sizes)
-    return (Route(parts[0].view(tokens, k), *parts[1:4]), parts[4].data_ptr() if need.value else None, need.value)
+    route = Route(parts[0].view(tokens, k), parts[1], parts[2], parts[3])
+    return route, parts[4].data_ptr() if size else None, size
 
 
 def sort_tokens(expert_ids: torch.Tensor, num_experts: int, align: int = 1, stream=None) -> Route:

@@ -384,7 +384,9 @@ int gp_add(size_t n, const float *a, const float *b, float *y, gp_stream s);
 /* Rows of the grouped layout: tokens * k and align - 1 for every expert that
  * can have a row, rounded down to whole groups. */
 int gp_route_rows(size_t tokens, size_t k, size_t experts, size_t align, size_t *rows);
-/* Device scratch of one gp_route_sort (0 for a short one, which may pass NULL). */
+/* Device scratch of one gp_route_sort: none, and NULL will do, up to
+ * GP_ROUTE_UNCOUNTED choices. */
+#define GP_ROUTE_UNCOUNTED 16384
 int gp_route_workspace(size_t tokens, size_t k, size_t experts, size_t *bytes);
 /* The layout of `ids` (device, id_bits 32 or 64, signed).  position: tokens * k,
  * order: gp_route_rows(), counts: experts, offsets: experts + 1 entries. */
@@ -397,7 +399,8 @@ int gp_route_dispatch(void *out, size_t out_stride, const void *x, size_t x_stri
                       const int32_t *position, const int32_t *order, size_t tokens, size_t k, size_t rows,
                       size_t width, gp_stream s);
 /* gp_route_sort, then gp_route_dispatch of the gp_route_rows() rows: one launch
- * up to 1024 choices. */
+ * up to 1024 choices; and up to GP_ROUTE_UNCOUNTED of them where tokens
+ * and rows are within 96 MiB. */
 int gp_route_sort_dispatch(void *out, size_t out_stride, const void *x, size_t x_stride, int type, const void *ids,
                            int id_bits, size_t tokens, size_t k, size_t experts, size_t align, size_t width,
                            int32_t *position, int32_t *order, int32_t *counts, int32_t *offsets, void *workspace,
