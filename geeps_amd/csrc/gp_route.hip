@@ -221,17 +221,13 @@ constexpr int kMoveWaves = kMoveBlock / kWave;
 constexpr unsigned kZeroRows = 16;  // places that one wave looks through for rows to clear
 
 // Rows are read and written once, so they go past the caches (non-temporal):
-// 8192 tokens of 4096 bf16, 8 choices: dispatch 109 us, 125 through them, combine
-// 103, 111 with its loads through them.  But
-//  - loads and dispatch's stores of rows that start off a 16-byte boundary go
-//    through them: two of a wave's accesses share a line there (32768 tokens of
-//    1001 fp16, 10 choices: dispatch 203 us, 237 past the caches);
-//  - combine_grad's stores do, where all of its rows fit the memory-side cache
-//    (8192 tokens of 2048 bf16, 8 choices: 90 us, 103 past it; 12000 tokens: 152,
-//    149 past it), and combine's, where the rows do not fit and leave it to y
-//    (16384 tokens of 4096 bf16: 205 us, 212 past it; 8192 of 2048: 52, 52).
-constexpr size_t kCachedRows = (size_t)256 << 20;
-
+// 8192 tokens of 2048 bf16, 8 choices: combine 52 us, 56 with its loads through
+// them; its gradient 103, 114 with its stores through them; dispatch of 4096, 6
+// choices: 91, 105.  But two waves' accesses share a line where rows do not start
+// at one: dispatch's stores then go through the caches (32768 tokens of 1001 fp16,
+// 10 choices: 210 us, 235 past them; 16384 of 600 bf16, 8 choices: 55, 57), and so
+// do loads from 2, 4, ... bytes off a 16-byte boundary (the gradient of 4099
+// tokens of 1001 floats: 22 us, 27 past them).
 struct Shape {
   unsigned tokens, k, rows, width;
   unsigned splits;       // waves that share a token's columns
@@ -333,7 +329,7 @@ __device__ __forceinline__ bool row_empty(const SortShared<W> &s, int r, int exp
 // calls.  16 tokens of 4096 bf16, 4 choices: see the host side.
 constexpr unsigned kSmallRoute = 1024;
 
-template <typename E, typename I, bool NT>
+template <typename E, typename I>
 __global__ __launch_bounds__(kMoveBlock) void route_sort_dispatch_kernel(
     E *__restrict__ out, size_t out_stride, const E *__restrict__ x, size_t x_stride, const I *__restrict__ ids,
     int experts, int bits, int align, int *__restrict__ position, int *__restrict__ order, int *__restrict__ counts,
@@ -372,20 +368,20 @@ __global__ __launch_bounds__(kMoveBlock) void route_sort_dispatch_kernel(
     const unsigned first = (wave - d.token_waves) * kZeroRows, r = first + lane;
     const bool empty = lane < (int)kZeroRows && r < d.rows && row_empty(s, (int)r, experts);
     if (empty) order[r] = -1;
-    clear_rows<E, NT>(out, out_stride, first, empty, d.width);
+    clear_rows<E, true>(out, out_stride, first, empty, d.width);
     return;
   }
   const unsigned t = wave / d.splits;
   const int p = lane < (int)d.k ? place[t * d.k + lane] : -1;
   const unsigned split = wave % d.splits;
   const E *row = x + (size_t)t * x_stride;
-  dispatch_token<E, NT>(out, out_stride, row, p, split, d, first_values(row, split, d));
+  dispatch_token<E, true>(out, out_stride, row, p, split, d, first_values(row, split, d));
 }
 
 // More choices: a block makes the places of its own share of the tokens and
 // moves them, two blocks to a CU, so the places cost no launch and no pass over
 // them of their own.  4099 tokens of 1001 floats, 3 choices: see the host side.
-template <typename E, typename I>
+template <typename E, typename I, bool NT>
 __global__ __launch_bounds__(kSortBlock) void route_place_dispatch_kernel(
     E *__restrict__ out, size_t out_stride, const E *__restrict__ x, size_t x_stride, const I *__restrict__ ids,
     int experts, int bits, int align, const int *__restrict__ hist, unsigned per_hist, unsigned hist_parts,
@@ -435,7 +431,7 @@ __global__ __launch_bounds__(kSortBlock) void route_place_dispatch_kernel(
       next_p = places_of(next);
       next_v = first_values(row_of(next), next % d.splits, d);
     }
-    dispatch_token<E, false>(out, out_stride, row_of(u), p, u % d.splits, d, v);
+    dispatch_token<E, NT>(out, out_stride, row_of(u), p, u % d.splits, d, v);
     p = next_p;
     v = next_v;
   }
@@ -445,7 +441,7 @@ __global__ __launch_bounds__(kSortBlock) void route_place_dispatch_kernel(
     const unsigned r = r0 + lane;
     const bool empty = lane < (int)kPer && r < d.rows && row_empty(s, (int)r, experts);
     if (empty) order[r] = -1;
-    clear_rows<E, false>(out, out_stride, r0, empty, d.width);
+    clear_rows<E, NT>(out, out_stride, r0, empty, d.width);
   }
 }
 
@@ -479,7 +475,7 @@ __device__ __forceinline__ void combine_group(typename Vec<E>::F &acc, uint64_t 
   for (int g = 0; g < G; ++g) acc += f[g] * to_float<E>(v[g]);  // choices in order, in 32 bits
 }
 
-template <typename E, bool NT, bool NT_OUT>
+template <typename E, bool NT>
 __global__ __launch_bounds__(kMoveBlock) void route_combine_kernel(E *__restrict__ y, size_t y_stride,
                                                                    const E *__restrict__ rows, size_t row_stride,
                                                                    const int *__restrict__ position,
@@ -505,7 +501,7 @@ __global__ __launch_bounds__(kMoveBlock) void route_combine_kernel(E *__restrict
     if (n >= 2) combine_group<E, 2, NT>(acc, left, rows, row_stride, p, w, c, whole, d.width), n -= 2;
     if (n >= 1) combine_group<E, 1, NT>(acc, left, rows, row_stride, p, w, c, whole, d.width);
     if (whole)
-      store_raw<E, NT_OUT>(to + c, from_float<E>(acc));
+      store_raw<E, true>(to + c, from_float<E>(acc));
     else
       store_part(to + c, from_float<E>(acc), d.width - c);
   }
@@ -517,7 +513,7 @@ __global__ __launch_bounds__(kMoveBlock) void route_combine_kernel(E *__restrict
 // are 32-bit sums, lane by lane, then over the wave, then over the splits' waves
 // in their order.
 // ---------------------------------------------------------------------------
-template <typename E, int G, bool NT, bool NT_OUT>
+template <typename E, int G, bool NT>
 __device__ __forceinline__ void grad_group(uint64_t &left, E *__restrict__ d_rows, size_t d_stride,
                                            const E *__restrict__ dy, const E *__restrict__ rows, size_t row_stride,
                                            int p, float w, unsigned first, unsigned step, unsigned width, float &dot) {
@@ -552,7 +548,7 @@ __device__ __forceinline__ void grad_group(uint64_t &left, E *__restrict__ d_row
       E *row = d_rows + at[g] * d_stride + c;
       const typename V::Raw out = from_float<E>(f[g] * o);
       if (whole)
-        store_raw<E, NT_OUT>(row, out);
+        store_raw<E, true>(row, out);
       else
         store_part(row, out, part);
     }
@@ -565,7 +561,7 @@ __device__ __forceinline__ void grad_group(uint64_t &left, E *__restrict__ d_row
 }
 
 // S waves share a token (d.splits = S); a block holds kMoveWaves / S tokens.
-template <typename E, int S, bool NT, bool NT_OUT>
+template <typename E, int S, bool NT>
 __global__ __launch_bounds__(kMoveBlock) void route_combine_grad_kernel(
     E *__restrict__ d_rows, size_t d_stride, void *__restrict__ d_weights, const E *__restrict__ dy, size_t dy_stride,
     const E *__restrict__ rows, size_t row_stride, const int *__restrict__ position, const int *__restrict__ order,
@@ -580,7 +576,7 @@ __global__ __launch_bounds__(kMoveBlock) void route_combine_grad_kernel(
     const unsigned first = (wave - d.token_waves) * kZeroRows, at = first + lane;
     const bool look = lane < (int)kZeroRows && at < d.rows;
     const int o = look ? order[at] : 0;
-    clear_rows<E, NT_OUT>(d_rows, d_stride, first, look && (o < 0 || (unsigned)o >= d.tokens * d.k), d.width);
+    clear_rows<E, true>(d_rows, d_stride, first, look && (o < 0 || (unsigned)o >= d.tokens * d.k), d.width);
   }
   const unsigned t = wave / S, split = wave % S;
   const size_t a = (size_t)t * d.k + lane;
@@ -594,10 +590,10 @@ __global__ __launch_bounds__(kMoveBlock) void route_combine_grad_kernel(
     const unsigned first = (split * kWave + lane) * V::N, step = S * kWave * V::N;
     uint64_t left = held;
     int n = __popcll(held);
-    for (; n >= 8; n -= 8) grad_group<E, 8, NT, NT_OUT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot);
-    if (n >= 4) grad_group<E, 4, NT, NT_OUT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot), n -= 4;
-    if (n >= 2) grad_group<E, 2, NT, NT_OUT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot), n -= 2;
-    if (n >= 1) grad_group<E, 1, NT, NT_OUT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot);
+    for (; n >= 8; n -= 8) grad_group<E, 8, NT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot);
+    if (n >= 4) grad_group<E, 4, NT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot), n -= 4;
+    if (n >= 2) grad_group<E, 2, NT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot), n -= 2;
+    if (n >= 1) grad_group<E, 1, NT>(left, d_rows, d_stride, o, rows, row_stride, p, w, first, step, d.width, dot);
   }
   if constexpr (S > 1) {
     part[in_block][lane] = dot;
@@ -633,13 +629,13 @@ constexpr size_t kMostSortBlocks = 1024;
 // places also move the tokens: the launch that it saves is worth more than the
 // blocks' fixed shares of the tokens cost.  In one launch (more than 16384
 // choices: two), and in one more:
-//   4099 tokens of 1001 floats, 3 choices (66 MB)   21.9 us, 27.4
-//   700 of 7168 bf16, 6 choices (70 MB)             26.8 us, 33.7
-//   2000 of 2048 bf16, 8 choices (74 MB)            38.0 us, 50.3
-//   4000 of 2048 bf16, 4 choices (82 MB)            22.4 us, 23.7
-//   6000 of 2048 bf16, 4 choices (123 MB)           26.8 us, 27.5
-//   10000 of 4000 bf16, 1 choice (160 MB)           39.0 us, 32.3
-//   8192 of 2048 bf16, 6 choices (235 MB)           53.6 us, 46.0
+//   4099 tokens of 1001 floats, 3 choices (66 MB)   22.0 us, 27.5
+//   700 of 7168 bf16, 6 choices (70 MB)             30.3 us, 33.0
+//   2000 of 2048 bf16, 8 choices (74 MB)            47.6 us, 51.2
+//   4000 of 2048 bf16, 4 choices (82 MB)            22.9 us, 24.2
+//   6000 of 2048 bf16, 4 choices (123 MB)           28.1 us, 27.6
+//   10000 of 4000 bf16, 1 choice (160 MB)           35.3 us, 32.3
+//   8192 of 2048 bf16, 6 choices (235 MB)           47.2 us, 46.0
 constexpr size_t kPlaceAndMove = (size_t)96 << 20;
 
 struct SortPlan {
@@ -703,9 +699,11 @@ unsigned pick_splits(size_t tokens, size_t width, int type, size_t least) {
   return (unsigned)(s < steps ? s : (steps ? steps : 1));
 }
 
-bool rows_aligned(const void *p, size_t stride, int type) {
-  return ((reinterpret_cast<uintptr_t>(p) | stride * type_size(type)) & 15) == 0;
+// Every row starts on a boundary of `bytes`.
+bool rows_start_at(size_t bytes, const void *p, size_t stride, int type) {
+  return ((reinterpret_cast<uintptr_t>(p) | stride * type_size(type)) & (bytes - 1)) == 0;
 }
+constexpr size_t kLine = 128;
 
 int check_grid(size_t waves, size_t *blocks) {
   GP_REQUIRE(waves <= UINT32_MAX, "too many rows for one call");
@@ -832,7 +830,7 @@ int gp_route_dispatch(void *out, size_t out_stride, const void *x, size_t x_stri
                            static_cast<const E *>(x), x_stride, position, order, d);
       });
     };
-    if (rows_aligned(out, out_stride, type))
+    if (rows_start_at(kLine, out, out_stride, type))
       go(route_dispatch_kernel<E, true>);
     else
       go(route_dispatch_kernel<E, false>);
@@ -868,27 +866,27 @@ int gp_route_sort_dispatch(void *out, size_t out_stride, const void *x, size_t x
       using I = decltype(id);
       const I *in = static_cast<const I *>(ids);
       if (n <= kSmallRoute) {
-        auto small = [&](auto kernel) {
-          launch_moves(blocks, d, [&](dim3 grid, Shape d) {
-            hipLaunchKernelGGL(kernel, grid, dim3(kMoveBlock), 0, (hipStream_t)s, static_cast<E *>(out), out_stride,
-                               static_cast<const E *>(x), x_stride, in, (int)experts, p.bits, (int)align, position,
-                               order, counts, offsets, d);
-          });
-        };
-        if (rows_aligned(out, out_stride, type))
-          small(route_sort_dispatch_kernel<E, I, true>);
-        else
-          small(route_sort_dispatch_kernel<E, I, false>);
+        launch_moves(blocks, d, [&](dim3 grid, Shape d) {
+          hipLaunchKernelGGL((route_sort_dispatch_kernel<E, I>), grid, dim3(kMoveBlock), 0, (hipStream_t)s,
+                             static_cast<E *>(out), out_stride, static_cast<const E *>(x), x_stride, in, (int)experts,
+                             p.bits, (int)align, position, order, counts, offsets, d);
+        });
         return;
       }
       if (p.counted)
         hipLaunchKernelGGL((route_count_kernel<I>), dim3(p.blocks), dim3(kSortBlock), 0, (hipStream_t)s, in,
                            (unsigned)n, p.per_block, (int)experts, hist);
       const size_t most = (size_t)device_cus() * 2;
-      hipLaunchKernelGGL((route_place_dispatch_kernel<E, I>), dim3((unsigned)(tokens < most ? tokens : most)),
-                         dim3(kSortBlock), 0, (hipStream_t)s, static_cast<E *>(out), out_stride,
-                         static_cast<const E *>(x), x_stride, in, (int)experts, p.bits, (int)align,
-                         (const int *)hist, p.per_block, p.blocks, position, order, counts, offsets, d);
+      auto move = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(tokens < most ? tokens : most)), dim3(kSortBlock), 0,
+                           (hipStream_t)s, static_cast<E *>(out), out_stride, static_cast<const E *>(x), x_stride, in,
+                           (int)experts, p.bits, (int)align, (const int *)hist, p.per_block, p.blocks, position, order,
+                           counts, offsets, d);
+      };
+      if (rows_start_at(kLine, out, out_stride, type))
+        move(route_place_dispatch_kernel<E, I, true>);
+      else
+        move(route_place_dispatch_kernel<E, I, false>);
     };
     id_bits == 64 ? go((int64_t)0) : go((int32_t)0);
   });
@@ -921,12 +919,10 @@ int gp_route_combine(void *y, size_t y_stride, const void *rows_in, size_t row_s
                            static_cast<const E *>(rows_in), row_stride, position, weights, wt, d);
       });
     };
-    if (!rows_aligned(rows_in, row_stride, type))
-      go(route_combine_kernel<E, false, true>);
-    else if (rows * width * type_size(type) > kCachedRows && rows_aligned(y, y_stride, type))
-      go(route_combine_kernel<E, true, false>);
+    if (rows_start_at(16, rows_in, row_stride, type))
+      go(route_combine_kernel<E, true>);
     else
-      go(route_combine_kernel<E, true, true>);
+      go(route_combine_kernel<E, false>);
   });
   GP_HIP_TRY(hipGetLastError());
   return GP_OK;
@@ -948,12 +944,16 @@ int gp_route_combine_grad(void *d_rows, size_t d_stride, void *d_weights, const 
   GP_REQUIRE(!bytes_overlap(d_rows, db, dy, yb), "d_rows overlaps dy");
   GP_REQUIRE(!bytes_overlap(d_rows, db, rows_in, rb), "d_rows overlaps the rows");
   const int wt = weight_type == GP_F32 ? kFloatWeights : kRowWeights;
-  // a token's waves meet for its weights' gradients: four, a block, or one.
-  // Short rows off a 16-byte boundary go to one wave (1001 floats: 22 us, 27
-  // with four), as do rows of one step.
-  const bool aligned = rows_aligned(rows_in, row_stride, type);
-  const size_t step = kWave * 16 / type_size(type);
-  const unsigned splits = width <= step || (!aligned && width <= 4 * step && tokens >= 4096) ? 1 : 4;
+  // A token's waves meet for its weights' gradients: four, a block (16384 tokens
+  // of 1000 floats, 4 choices: 99 us, 105 with two, 113 with one); two where the
+  // row has two steps for them (16384 of 600 bf16, 8 choices: 72 us, 88 with
+  // four); one for short rows off a 16-byte boundary, whose lines they would
+  // share (8192 of 1001 bf16, 3 choices: 26 us, 28 with two, 40 with four; not
+  // for few tokens), and for rows of one step.
+  const bool aligned = rows_start_at(16, rows_in, row_stride, type);
+  const size_t step = kWave * 16 / type_size(type), steps = (width + step - 1) / step;
+  const bool one = steps <= 1 || (!aligned && steps <= 4 && tokens >= 4096);
+  const unsigned splits = one ? 1 : steps == 2 ? 2 : 4;
   Shape d{(unsigned)tokens, (unsigned)k, (unsigned)rows, (unsigned)width, splits, 0, 0};
   const size_t waves = tokens * (size_t)d.splits;
   size_t blocks = 0;
@@ -970,15 +970,15 @@ int gp_route_combine_grad(void *d_rows, size_t d_stride, void *d_weights, const 
     };
     auto pick = [&](auto s) {
       constexpr int S = decltype(s)::value;
-      if (!aligned)
-        go(route_combine_grad_kernel<E, S, false, true>);
-      else if (rows * width * type_size(type) <= kCachedRows)
-        go(route_combine_grad_kernel<E, S, true, false>);
+      if (aligned)
+        go(route_combine_grad_kernel<E, S, true>);
       else
-        go(route_combine_grad_kernel<E, S, true, true>);
+        go(route_combine_grad_kernel<E, S, false>);
     };
     if (splits == 4)
       pick(std::integral_constant<int, 4>());
+    else if (splits == 2)
+      pick(std::integral_constant<int, 2>());
     else
       pick(std::integral_constant<int, 1>());
   });
