@@ -272,9 +272,11 @@ __global__ __launch_bounds__(kClipBlock) void sum_square_kernel(float *__restric
   }
 }
 
-// out = in + f * (b0 + ... + b{NB-1}); one bucket also serves a sum that was left.
-// All of it past the caches: one stream of 61 M floats 124 us, 136 through them.
-template <int NB>
+// out = in + f * (b0 + ... + b{NB-1}); LEFT: b0 is the sum that the first pass
+// left, partly still in the memory-side cache, and is read through the caches
+// (61 M floats of three buckets: both passes 255 us, 271 past them), all else
+// past them (one stream of 61 M floats: this pass 124 us, 136 through them).
+template <int NB, bool LEFT>
 __global__ __launch_bounds__(kClipBlock) void add_scaled_kernel(float *__restrict__ out, const float *__restrict__ in,
                                                                 Streams b, size_t n,
                                                                 const double *__restrict__ partial, unsigned partials,
@@ -291,7 +293,7 @@ __global__ __launch_bounds__(kClipBlock) void add_scaled_kernel(float *__restric
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[j][u] = load_raw<float, true>(b.p[j] + i + u * kClipBlock * 4);
+        for (int u = 0; u < U; ++u) v[j][u] = load_raw<float, !LEFT>(b.p[j] + i + u * kClipBlock * 4);
 #pragma unroll
       for (int u = 0; u < U; ++u) m[u] = load_raw<float, true>(in + i + u * kClipBlock * 4);
 #pragma unroll
@@ -620,12 +622,15 @@ int gp_bucket_sum_clipped(float *out, const float *in, const float *const *bucke
   if (num_buckets == 2) st.p[1] = buckets[1];
   const dim3 grid(clip_grid((num_vals + kClipBlock * 16 - 1) / (kClipBlock * 16))), block(kClipBlock);
   const double *from = sum ? sum : partial;
-  if (num_buckets == 2)
-    hipLaunchKernelGGL((add_scaled_kernel<2>), grid, block, 0, (hipStream_t)s, out, in, st, num_vals, from, partials,
-                       b, norm);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, block, 0, (hipStream_t)s, out, in, st, num_vals, from, partials, b, norm);
+  };
+  if (!reread)
+    go(add_scaled_kernel<1, true>);
+  else if (num_buckets == 2)
+    go(add_scaled_kernel<2, false>);
   else
-    hipLaunchKernelGGL((add_scaled_kernel<1>), grid, block, 0, (hipStream_t)s, out, in, st, num_vals, from, partials,
-                       b, norm);
+    go(add_scaled_kernel<1, false>);
   GP_HIP_TRY(hipGetLastError());
   return GP_OK;
 }
