@@ -66,7 +66,9 @@ class GradPlan:
     compiled once (gp_grad_plan_create, outside of any graph capture), for buffers
     that stay in place from step to step.  ``outs`` (default: the gradients themselves) are of the gradients'
     types or float32, and overlap nothing but, each, its own gradient.  The plan
-    keeps the tensors; replacing one of them takes a new plan."""
+    keeps the tensors; replacing one of them takes a new plan.  A captured graph of
+    its calls needs the plan, which holds the table of buffers on the device, for
+    as long as it is replayed."""
 
     def __init__(self, grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor] | None = None):
         self._h = ctypes.c_void_p()

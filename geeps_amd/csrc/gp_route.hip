@@ -395,7 +395,7 @@ __global__ __launch_bounds__(kSortBlock) void route_place_dispatch_kernel(
   const unsigned per_wave = (hi - lo + kSortBlock - 1) / kSortBlock * kWave;
   const unsigned from = min(hi, lo + wave * per_wave), to = min(hi, from + per_wave);
   int key = from + lane < to ? key_of(ids[from + lane], experts) : experts;
-  route_prepare(s, key, ids, n, lo, from, to, gridDim.x == 1, experts, align, hist, per_hist, hist_parts);
+  route_prepare(s, key, ids, n, lo, from, to, false, experts, align, hist, per_hist, hist_parts);
   for (unsigned i0 = from; i0 < to; i0 += kWave) {
     const unsigned i = i0 + lane;
     if (i0 != from) key = i < to ? key_of(ids[i], experts) : experts;

@@ -443,3 +443,54 @@ def test_sort_and_dispatch_few_choices(dev, id_type, tokens, k, experts, align, 
         held = route.order >= 0
         assert torch.equal(out[:len(want[1])][held], x[route.order[held].long() // k])
         assert not bool(out[:len(want[1])][~held].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,tokens,k,experts,align,width", [
+    (torch.bfloat16, 17, 64, 64, 1, 24), (torch.float32, 1025, 1, 1, 64, 1), (torch.float16, 513, 3, 1024, 3, 130),
+    (torch.bfloat16, 5461, 3, 60, 16, 128), (torch.float32, 16385, 1, 300, 8, 33), (torch.bfloat16, 6001, 3, 1024, 1, 64),
+    (torch.float16, 9001, 7, 5, 32, 72), (torch.bfloat16, 600, 2, 9, 1, 5001)])
+def test_sort_and_dispatch_more_choices(dev, dtype, tokens, k, experts, align, width):
+    """Places and moves in one launch: with every block's own count, and past 16384 choices with counts in runs."""
+    r = np.random.default_rng(tokens)
+    for kind in ("any", "last first", "one", "none"):
+        if kind == "any":
+            ids = r.integers(-2, experts + 2, (tokens, k))
+        elif kind == "last first":  # the groups' order is the tokens' backwards
+            ids = np.sort(r.integers(0, experts, (tokens, k)), axis=0)[::-1].copy()
+        else:
+            ids = np.full((tokens, k), experts - 1 if kind == "one" else experts)
+        want = places(np.where((ids >= 0) & (ids < experts), ids, -1), experts, align)
+        n = len(want[1])
+        x = as_device((tokens, width), dtype, dev, 1)
+        wide = as_device((n + 5, width + 3), dtype, dev, 2)  # rows of another stride, at an odd place
+        before, out = wide.clone(), wide[:, 2:2 + width]
+        rows, route = routing.sort_and_dispatch(x, torch.from_numpy(ids).to(dev), experts, align, out=out)
+        plain, again = routing.sort_and_dispatch(x, torch.from_numpy(ids).int().to(dev), experts, align)
+        same_route(route, want)
+        same_route(again, want)
+        held = route.order >= 0
+        assert torch.equal(plain[held], x[route.order[held].long() // k]) and not bool(plain[~held].any())
+        assert rows is out and torch.equal(out[:n], plain)
+        before[:n, 2:2 + width] = plain
+        assert torch.equal(wide, before)
+
+
+@pytest.mark.gpu
+def test_more_waves_than_a_grid_holds(dev):
+    """2^26 tokens: more than 2^32 lanes."""
+    tokens = (1 << 26) + 1003
+    ids = (torch.arange(tokens, device=dev, dtype=torch.int32) * 7919 % 5 - 1).view(-1, 1)
+    x = (torch.arange(tokens, device=dev, dtype=torch.int32) % 2039).to(torch.float16).view(-1, 1)
+    rows, route = routing.sort_and_dispatch(x, ids, 4)
+    p = route.position.view(-1)
+    held = p >= 0
+    assert torch.equal(held, (ids >= 0).view(-1)) and int(route.counts.sum()) == int(held.sum())
+    at = route.order.long().clamp(min=0)
+    assert torch.equal(rows.view(-1), torch.where(route.order >= 0, x.view(-1)[at], torch.zeros((), dtype=x.dtype, device=dev)))
+    y = routing.combine(rows, route)
+    assert torch.equal(y.view(-1), torch.where(held, x.view(-1), torch.zeros((), dtype=x.dtype, device=dev)))
+    w = torch.full((tokens, 1), 2.0, device=dev)
+    d_rows, d_w = routing.combine_grad(x, rows, route, w)
+    assert torch.equal(d_rows, 2 * rows)
+    assert torch.equal(d_w.view(-1), torch.where(held, x.view(-1).float() ** 2, torch.zeros((), device=dev)))
