@@ -218,7 +218,10 @@ __global__ __launch_bounds__(kSortBlock) void route_place_kernel(
 // ---------------------------------------------------------------------------
 constexpr int kMoveBlock = 256;
 constexpr int kMoveWaves = kMoveBlock / kWave;
-constexpr unsigned kZeroRows = 16;  // places that one wave looks through for rows to clear
+// Places that one wave looks through for rows to clear: a dispatch of 8192 tokens
+// of 4096 bf16 with 20000 rows of padding 172 us, 180 with sixteen, 173 with one;
+// the gradient of 8192 of 2048, 64 experts in groups of 16, 104, 105 and 109.
+constexpr unsigned kZeroRows = 4;
 
 // Rows are read and written once, so they go past the caches (non-temporal):
 // 8192 tokens of 2048 bf16, 8 choices: combine 52 us, 56 with its loads through
@@ -326,7 +329,8 @@ __device__ __forceinline__ bool row_empty(const SortShared<W> &s, int r, int exp
 
 // Few choices: every block makes the places for itself, in LDS, and moves its
 // own tokens, in one launch.  The first block leaves the places for later
-// calls.  16 tokens of 4096 bf16, 4 choices: see the host side.
+// calls.  Bound by the launch: 16 tokens of 4096 bf16, 4 choices, 4.5 us on the
+// device in a pass of 12.7; 21.9 a pass with the places in a launch of their own.
 constexpr unsigned kSmallRoute = 1024;
 
 template <typename E, typename I>
@@ -380,7 +384,8 @@ __global__ __launch_bounds__(kMoveBlock) void route_sort_dispatch_kernel(
 
 // More choices: a block makes the places of its own share of the tokens and
 // moves them, two blocks to a CU, so the places cost no launch and no pass over
-// them of their own.  4099 tokens of 1001 floats, 3 choices: see the host side.
+// them of their own (kPlaceAndMove: where, and what it measured).  Bound by HBM:
+// 4099 tokens of 1001 floats, 3 choices, 68 MB in 20.4 us a pass.
 template <typename E, typename I, bool NT>
 __global__ __launch_bounds__(kSortBlock) void route_place_dispatch_kernel(
     E *__restrict__ out, size_t out_stride, const E *__restrict__ x, size_t x_stride, const I *__restrict__ ids,
@@ -435,11 +440,10 @@ __global__ __launch_bounds__(kSortBlock) void route_place_dispatch_kernel(
     p = next_p;
     v = next_v;
   }
-  // rows that hold no choice: kPer of them to a wave at a time
-  constexpr unsigned kPer = 4;
-  for (unsigned r0 = (blockIdx.x * kSortWaves + wave) * kPer; r0 < d.rows; r0 += gridDim.x * kSortWaves * kPer) {
+  // rows that hold no choice
+  for (unsigned r0 = (blockIdx.x * kSortWaves + wave) * kZeroRows; r0 < d.rows; r0 += gridDim.x * kSortWaves * kZeroRows) {
     const unsigned r = r0 + lane;
-    const bool empty = lane < (int)kPer && r < d.rows && row_empty(s, (int)r, experts);
+    const bool empty = lane < (int)kZeroRows && r < d.rows && row_empty(s, (int)r, experts);
     if (empty) order[r] = -1;
     clear_rows<E, NT>(out, out_stride, r0, empty, d.width);
   }
