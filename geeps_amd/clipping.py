@@ -57,8 +57,10 @@ def _total(total, device):
     return total.data_ptr()
 
 
-def _workspace(device):
-    return torch.empty(native.GP_CLIP_WORKSPACE_BYTES // 8, dtype=torch.float64, device=device)
+def _workspace(like):
+    """A call's workspace, on a float32 tensor's device.  The caller holds it until
+    the call has returned: another thread may allocate on the same stream."""
+    return like.new_empty(native.GP_CLIP_WORKSPACE_BYTES // 4)
 
 
 class GradPlan:
@@ -90,6 +92,9 @@ class GradPlan:
         with torch.cuda.device(self.device):
             if torch.cuda.is_current_stream_capturing():
                 raise ValueError("a plan cannot be made while a graph is captured: its table is copied to the device")
+            # what a call allocates: the norm and a workspace, each call's own
+            self._like = (torch.empty((), dtype=torch.float32, device=self.device),
+                          torch.empty(native.GP_CLIP_WORKSPACE_BYTES // 4, dtype=torch.float32, device=self.device))
         n = len(self.grads)
         ptrs, ints, sizes = ctypes.c_void_p * n, ctypes.c_int * n, ctypes.c_size_t * n
         with torch.cuda.device(self.device):
@@ -110,7 +115,8 @@ class GradPlan:
             with _On(self.device, stream):
                 return self.sum_squares()
         total = torch.empty((), dtype=torch.float64, device=self.device)
-        check(native.lib().gp_grad_sum_squares(self._h, total.data_ptr(), _workspace(self.device).data_ptr(),
+        workspace = torch.empty_like(self._like[1])
+        check(native.lib().gp_grad_sum_squares(self._h, total.data_ptr(), workspace.data_ptr(),
                                                _current_stream(self.device.index)), "gp_grad_sum_squares")
         return total
 
@@ -132,10 +138,9 @@ class GradPlan:
         if stream is not None or self.device.index != _current_device():
             with _On(self.device, stream):
                 return self.clip(max_norm, scale, total, skip_nonfinite)
-        norm = torch.empty((), dtype=torch.float32, device=self.device)
-        check(native.lib().gp_grad_clip(self._h, max_norm, scale, mode, given, norm.data_ptr(),
-                                        _workspace(self.device).data_ptr(), _current_stream(self.device.index)),
-              "gp_grad_clip")
+        norm, workspace = torch.empty_like(self._like[0]), torch.empty_like(self._like[1])
+        check(native.lib().gp_grad_clip(self._h, max_norm, scale, mode, given, norm.data_ptr(), workspace.data_ptr(),
+                                        _current_stream(self.device.index)), "gp_grad_clip")
         return norm
 
     def close(self) -> None:
@@ -184,9 +189,9 @@ def sum_updates_squares(updates: Sequence[torch.Tensor], scratch: torch.Tensor |
             return sum_updates_squares(updates, scratch)
     ptrs = _buckets(updates, n, device)
     scratch = _scratch(scratch, len(updates), n, device)
-    total = torch.empty((), dtype=torch.float64, device=device)
+    total, workspace = torch.empty((), dtype=torch.float64, device=device), _workspace(updates[0])
     check(native.lib().gp_bucket_sum_squares(None if scratch is None else scratch.data_ptr(), ptrs, len(updates), n,
-                                             total.data_ptr(), _workspace(device).data_ptr(),
+                                             total.data_ptr(), workspace.data_ptr(),
                                              _current_stream(device.index)), "gp_bucket_sum_squares")
     return total
 
@@ -219,9 +224,9 @@ def apply_updates_clipped(master: torch.Tensor, updates: Sequence[torch.Tensor],
     if given is not None and scratch is None and len(updates) > 2:
         raise ValueError("total needs the scratch that sum_updates_squares left")
     scratch = _scratch(scratch, len(updates), n, device)
-    norm = torch.empty((), dtype=torch.float32, device=device)
+    norm, workspace = master.new_empty(()), _workspace(master)
     check(native.lib().gp_bucket_sum_clipped(out.data_ptr(), master.data_ptr(), ptrs, len(updates), n,
                                              None if scratch is None else scratch.data_ptr(), max_norm, bound_scale, mode,
-                                             given, norm.data_ptr(), _workspace(device).data_ptr(),
+                                             given, norm.data_ptr(), workspace.data_ptr(),
                                              _current_stream(device.index)), "gp_bucket_sum_clipped")
     return norm

@@ -463,3 +463,35 @@ def test_bound_is_over_all_shards(tmp_path, world, rows, width, clients, exchang
         assert abs(float(g["norm"]) - norm) <= 1.01 * (U * norm + clients * U * float(size.square().sum().sqrt()))
         bound = 2 * f * (2 * clients + 6) * U * (size + 2 * u.abs())
         assert bool(((g["table"].double() - 2 * f * u).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+def test_workspace_is_held_while_a_call_runs(dev, monkeypatch):
+    """No allocation of the same stream, made while a call runs, gets the call's workspace."""
+    real = native.lib()
+    sides = {"gp_grad_clip": 6, "gp_grad_sum_squares": 2, "gp_bucket_sum_clipped": 11, "gp_bucket_sum_squares": 5}
+    seen = []
+
+    class Watched:
+        def __getattr__(self, name):
+            f = getattr(real, name)
+            if name not in sides:
+                return f
+
+            def call(*args):
+                other = [torch.empty(native.GP_CLIP_WORKSPACE_BYTES, dtype=torch.uint8, device=dev) for _ in range(4)]
+                assert args[sides[name]] not in [t.data_ptr() for t in other], name
+                seen.append(name)
+                return f(*args)
+            return call
+
+    grads = [torch.randn(1000, device=dev), torch.randn(3, device=dev)]
+    plan = clipping.GradPlan(grads)
+    updates = [torch.randn(5000, device=dev) for _ in range(3)]
+    master = torch.zeros(5000, device=dev)
+    monkeypatch.setattr(native, "lib", lambda: Watched())
+    plan.clip(1.0)
+    plan.sum_squares()
+    clipping.apply_updates_clipped(master, updates, 1.0)
+    clipping.sum_updates_squares(updates)
+    assert sorted(seen) == sorted(sides)
