@@ -207,9 +207,11 @@ __global__ __launch_bounds__(kSortBlock) void route_place_kernel(
   }
   // places that hold no choice: the groups' padding, then all behind the last group
   const unsigned waves = gridDim.x * kSortWaves, me = blockIdx.x * kSortWaves + wave;
+  // (unsigned: a lane's place and the step after it may pass 2^31 near the most rows)
   if (align > 1)
     for (unsigned e = me; e < (unsigned)experts; e += waves)
-      for (int p = s.offset[e] + s.total[e] + lane; p < s.offset[e + 1]; p += kWave) order[p] = -1;
+      for (unsigned p = (unsigned)(s.offset[e] + s.total[e]) + lane; p < (unsigned)s.offset[e + 1]; p += kWave)
+        order[p] = -1;
   for (unsigned p = s.offset[experts] + me * kWave + lane; p < rows; p += waves * kWave) order[p] = -1;
 }
 
