@@ -68,9 +68,12 @@ class GradPlan:
     compiled once (gp_grad_plan_create, outside of any graph capture), for buffers
     that stay in place from step to step.  ``outs`` (default: the gradients themselves) are of the gradients'
     types or float32, and overlap nothing but, each, its own gradient.  The plan
-    keeps the tensors; replacing one of them takes a new plan.  A captured graph of
-    its calls needs the plan, which holds the table of buffers on the device, for
-    as long as it is replayed."""
+    keeps the tensors and their storages.  A tensor whose memory was replaced since
+    (``t.data = ...``, ``module.half()``, ``resize_``) makes every call raise
+    ValueError; it takes a new plan.  A captured graph of the plan's calls needs the
+    plan, which holds the table of buffers on the device and their memory, for as
+    long as it is replayed; a replay checks nothing, so its tensors keep their
+    memory until then."""
 
     def __init__(self, grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor] | None = None):
         self._h = ctypes.c_void_p()
@@ -95,6 +98,10 @@ class GradPlan:
             # what a call allocates: the norm and a workspace, each call's own
             self._like = (torch.empty((), dtype=torch.float32, device=self.device),
                           torch.empty(native.GP_CLIP_WORKSPACE_BYTES // 4, dtype=torch.float32, device=self.device))
+        # what the table points at: it must not be given to other tensors, and must be what the tensors still hold
+        self._tensors = (*self.grads, *(() if outs is None else self.outs))
+        self._storages = [t.untyped_storage() for t in self._tensors]
+        self._facts, self._moved = native.tensor_facts().facts(self._tensors), native.tensor_facts().moved
         n = len(self.grads)
         ptrs, ints, sizes = ctypes.c_void_p * n, ctypes.c_int * n, ctypes.c_size_t * n
         with torch.cuda.device(self.device):
@@ -107,6 +114,11 @@ class GradPlan:
     def _open(self):
         if not self._h:
             raise ValueError("the plan is closed")
+        moved = self._moved(self._tensors, self._facts)
+        if moved >= 0:
+            n = len(self.grads)
+            name = f"grads[{moved}]" if moved < n else f"outs[{moved - n}]"
+            raise ValueError(f"{name} is not where it was when the plan was made, or of another length or type")
 
     def sum_squares(self, stream=None) -> torch.Tensor:
         """The sum of the gradients' squares: one float64 value."""
@@ -147,7 +159,7 @@ class GradPlan:
         if self._h:
             native.lib().gp_grad_plan_destroy(self._h)
             self._h = ctypes.c_void_p()
-        self.grads = self.outs = ()
+        self.grads = self.outs = self._tensors = self._storages = ()
 
     def __del__(self):
         try:

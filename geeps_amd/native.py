@@ -7,12 +7,14 @@ no CPU fallback anywhere in the package.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import re
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libgp_reduce.so")
+FACTS_PATH = os.path.join(_HERE, "lib", "gp_tensors.so")
 HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "gp_reduce.h")
 
 GP_OK = 0
@@ -159,6 +161,7 @@ _SIGNATURES = {
 
 _lock = threading.Lock()
 _lib = None
+_facts = None
 
 
 def declared_symbols(header: str = HEADER_PATH) -> list[str]:
@@ -189,6 +192,21 @@ def lib() -> ctypes.CDLL:
             raise ImportError("geeps_amd: libgp_reduce.so ABI version mismatch")
         _lib = handle
         return _lib
+
+
+def tensor_facts():
+    """The module gp_tensors (csrc/gp_tensors.cpp): whether tensors are what and where they were."""
+    global _facts
+    if _facts is None:
+        if not os.path.exists(FACTS_PATH):
+            raise ImportError(f"geeps_amd: not built: {FACTS_PATH} is missing "
+                              "(run `python -c 'import __graft_entry__ as g; g.build()'`)")
+        import torch  # noqa: F401  its libraries, which the module's symbols come from
+        spec = importlib.util.spec_from_file_location("gp_tensors", FACTS_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _facts = module
+    return _facts
 
 
 def unplanned_stats() -> dict:
