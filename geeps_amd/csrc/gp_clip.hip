@@ -448,6 +448,9 @@ struct Span {
   size_t i;
 };
 
+// Beside one for each gradient's end: 2^40 values, more than the device's memory holds.
+constexpr size_t kMostChunks = (size_t)1 << 25;
+
 // Chunk length: a whole number of 16-byte steps of a block, long enough that
 // the table stays small, short enough that every block of the grid gets some.
 size_t chunk_length(size_t total) {
@@ -469,6 +472,7 @@ int build_grad_plan(gp_grad_plan_s *p, size_t count, const void *const *grads, c
     GP_REQUIRE(sizes[i] <= SIZE_MAX / 8, "gradient too long");
     const uintptr_t lo = reinterpret_cast<uintptr_t>(outs[i]);
     spans.push_back({lo, lo + sizes[i] * type_size(out_types[i]), i});
+    GP_REQUIRE(total <= SIZE_MAX / 8 - sizes[i], "gradients too long");
     total += sizes[i];
     p->bytes += sizes[i] * type_size(types[i]);
   }
@@ -485,13 +489,16 @@ int build_grad_plan(gp_grad_plan_s *p, size_t count, const void *const *grads, c
                  "an output overlaps a gradient and is not that gradient itself");
   }
   const size_t len = chunk_length(total);
+  size_t needed = 0;  // known before the table takes any memory: 32 bytes each
+  for (size_t i = 0; i < count; ++i) needed += sizes[i] / len + (sizes[i] % len != 0);
+  GP_REQUIRE(needed <= kMostChunks + count && needed <= (size_t)INT32_MAX, "too many values for one plan");
   std::vector<Chunk> chunks;
+  chunks.reserve(needed);
   for (size_t i = 0; i < count; ++i)
     for (size_t at = 0; at < sizes[i]; at += len)
       chunks.push_back({static_cast<const char *>(grads[i]) + at * type_size(types[i]),
                         static_cast<char *>(outs[i]) + at * type_size(out_types[i]),
                         (unsigned)std::min(len, sizes[i] - at), (short)types[i], (short)out_types[i]});
-  GP_REQUIRE(chunks.size() <= (size_t)INT32_MAX, "too many gradients for one plan");
   p->count = chunks.size();
   if (chunks.empty()) return GP_OK;
   GP_HIP_TRY(hipGetDevice(&p->device));
