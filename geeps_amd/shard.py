@@ -103,7 +103,9 @@ class ShardedReducer:
     hosted client ``hosted[j]``.  ``push()`` runs the exchange, ``apply()`` the
     device-resident N-way sum, ``refresh()`` the all-gather.  With ``max_norm``
     ``apply()`` bounds the norm of the whole table's summed update, over all
-    shards, and leaves it in ``norm`` (a device value, the same on every rank).
+    shards, and leaves it in ``norm`` (a device value, the same on every rank); a
+    client's NaN or infinity then goes into the table of every rank.  ``apply_fn``
+    takes no bound and is refused beside ``max_norm``, as ``clip_fns`` without it.
     """
 
     def __init__(self, num_rows: int, row_size: int, num_clients: int, device,
@@ -124,6 +126,10 @@ class ShardedReducer:
         self.apply_fn = apply_fn or _default_apply
         if max_norm is not None and not max_norm >= 0.0:
             raise ValueError("max_norm must not be negative or NaN")
+        if max_norm is not None and apply_fn is not None:
+            raise ValueError("apply_fn adds an update without a bound: with max_norm pass clip_fns")
+        if max_norm is None and clip_fns is not None:
+            raise ValueError("clip_fns are for a bounded update: pass max_norm")
         self.max_norm = max_norm
         self.squares_fn, self.clipped_fn = clip_fns or (_default_squares, _default_clipped)
         self.norm = None
