@@ -16,6 +16,11 @@ back from it: the grouped layout has a fixed number of rows.
     d_rows, d_weights = combine_grad(dy, rows, route, weights)
     dx = dispatch_grad(d_rows, route)
 
+Outputs carry no gradient: the calls for it are the two above, for a manual
+backward pass or an autograd.Function of them.  A tensor that requires one is
+refused while gradients are recorded, rather than cut off from its graph; under
+torch.no_grad() or inside a Function's forward it is taken.
+
 Every call can be captured into a HIP graph.  Rows are float32, bfloat16 or
 float16, one contiguous row after another or with a row stride; sums are kept in
 32 bits.  An id outside [0, num_experts) is a choice with no row (padding, or an
@@ -75,8 +80,16 @@ class _On:
             g.__exit__(*exc)
 
 
+def _no_gradient(t, name):
+    if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which the result would not carry: call this under "
+                         "torch.no_grad() or in an autograd.Function, with combine_grad and dispatch_grad for its "
+                         "backward pass")
+
+
 def _rows2d(t, name, dtype=None, device=None, width=None) -> int:
     """The row stride of a (rows, width) tensor, checked."""
+    _no_gradient(t, name)
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA (HIP) tensor")
     if t.dim() != 2:
@@ -224,6 +237,7 @@ def sort_and_dispatch(x: torch.Tensor, expert_ids: torch.Tensor, num_experts: in
 
 
 def _weights(weights, tokens, k, like) -> int:
+    _no_gradient(weights, "weights")
     if not isinstance(weights, torch.Tensor) or weights.device != like.device or not weights.is_contiguous():
         raise ValueError("weights must be a contiguous tensor on the rows' device")
     if weights.dtype not in (torch.float32, like.dtype):
