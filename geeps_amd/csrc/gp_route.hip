@@ -766,14 +766,28 @@ size_t strided_bytes(size_t rows, size_t stride, size_t width, int type) {
   return rows && width ? ((rows - 1) * stride + width) * type_size(type) : 0;
 }
 
+// Two sets of rows of one width share a value.  Rows of one stride, as columns of
+// one buffer are, lie in windows of it that repeat, and may pass between each
+// other; of two strides only the spans are looked at.
+bool rows_overlap(const void *a, size_t a_rows, size_t a_stride, const void *b, size_t b_rows, size_t b_stride,
+                  size_t width, int type) {
+  if (!bytes_overlap(a, strided_bytes(a_rows, a_stride, width, type), b, strided_bytes(b_rows, b_stride, width, type)))
+    return false;
+  if (a_rows == 1) a_stride = b_stride;  // a single row has any
+  if (b_rows == 1) b_stride = a_stride;
+  if (a_stride != b_stride) return true;
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  const size_t bytes = width * type_size(type), step = a_stride * type_size(type);
+  const size_t apart = x >= y ? (x - y) % step : (step - (y - x) % step) % step;  // from b's window to a's
+  return apart < bytes || step - apart < bytes;
+}
+
 int plan_dispatch(const void *out, size_t out_stride, const void *x, size_t x_stride, int type, size_t tokens,
                   size_t k, size_t rows, size_t width, Shape *d, size_t *blocks) {
   GP_TRY(check_move(tokens, k, rows, width, type));
   GP_REQUIRE(out && (tokens == 0 || x), "null out or x");
   GP_REQUIRE(out_stride >= width && x_stride >= width, "row stride smaller than the width");
-  GP_REQUIRE(!bytes_overlap(out, strided_bytes(rows, out_stride, width, type), x,
-                            strided_bytes(tokens, x_stride, width, type)),
-             "out overlaps x");
+  GP_REQUIRE(!rows_overlap(out, rows, out_stride, x, tokens, x_stride, width, type), "out overlaps x");
   *d = Shape{(unsigned)tokens, (unsigned)k, (unsigned)rows, (unsigned)width, pick_splits(tokens, width, type, k < 4 ? 8 : 4), 0, 0};
   const size_t waves = tokens * (size_t)d->splits;
   GP_TRY(check_grid(waves + (rows + kZeroRows - 1) / kZeroRows, blocks));
@@ -914,9 +928,7 @@ int gp_route_combine(void *y, size_t y_stride, const void *rows_in, size_t row_s
   if (tokens == 0 || width == 0) return GP_OK;
   GP_REQUIRE(y && position && (rows == 0 || rows_in), "null y, rows or position");
   GP_REQUIRE(y_stride >= width && row_stride >= width, "row stride smaller than the width");
-  GP_REQUIRE(!bytes_overlap(y, strided_bytes(tokens, y_stride, width, type), rows_in,
-                            strided_bytes(rows, row_stride, width, type)),
-             "y overlaps the rows");
+  GP_REQUIRE(!rows_overlap(y, tokens, y_stride, rows_in, rows, row_stride, width, type), "y overlaps the rows");
   const int wt = !weights ? kNoWeights : weight_type == GP_F32 ? kFloatWeights : kRowWeights;
   Shape d{(unsigned)tokens, (unsigned)k, (unsigned)rows, (unsigned)width, pick_splits(tokens, width, type, 8), 0, 0};
   const size_t waves = tokens * (size_t)d.splits;
@@ -951,10 +963,9 @@ int gp_route_combine_grad(void *d_rows, size_t d_stride, void *d_weights, const 
   GP_REQUIRE(rows == 0 || order, "null order");
   GP_REQUIRE(width == 0 || ((tokens == 0 || dy) && (rows == 0 || (d_rows && rows_in))), "null dy, rows or d_rows");
   GP_REQUIRE(d_stride >= width && dy_stride >= width && row_stride >= width, "row stride smaller than the width");
-  const size_t db = strided_bytes(rows, d_stride, width, type), rb = strided_bytes(rows, row_stride, width, type);
-  const size_t yb = strided_bytes(tokens, dy_stride, width, type);
-  GP_REQUIRE(!bytes_overlap(d_rows, db, dy, yb), "d_rows overlaps dy");
-  GP_REQUIRE(!bytes_overlap(d_rows, db, rows_in, rb), "d_rows overlaps the rows");
+  GP_REQUIRE(!rows_overlap(d_rows, rows, d_stride, dy, tokens, dy_stride, width, type), "d_rows overlaps dy");
+  GP_REQUIRE(!rows_overlap(d_rows, rows, d_stride, rows_in, rows, row_stride, width, type),
+             "d_rows overlaps the rows");
   const int wt = weight_type == GP_F32 ? kFloatWeights : kRowWeights;
   // A token's waves meet for its weights' gradients: four, a block (16384 tokens
   // of 1000 floats, 4 choices: 99 us, 105 with two, 113 with one); two where the
