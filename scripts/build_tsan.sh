@@ -14,7 +14,7 @@ mkdir -p "$OUT"
   -I"$REPO/include" -I"$REPO/geeps_amd/csrc/geeps" -shared -o "$OUT/libgeeps.so" \
   "$REPO"/geeps_amd/csrc/geeps/*.cpp -L"$REPO/geeps_amd/lib" -lgp_reduce \
   -Wl,-rpath,'$ORIGIN/../../geeps_amd/lib'
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O2 -std=c++17 -I "$REPO/include" -Xarch_host -fsanitize=thread \
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O2 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -I "$REPO/include" -Xarch_host -fsanitize=thread \
   "$REPO/tests/apps/geeps_sum_app.cpp" -o "$OUT/geeps_sum_app" -L"$OUT" -lgeeps \
   -Wl,-rpath,'$ORIGIN'
 echo "built $OUT"

@@ -39,6 +39,21 @@ def test_no_unit_is_built_with_packed_arithmetic():
         assert unit not in UNITS or "-Xclang -target-feature -Xclang -packed-fp32-ops" in line, unit
 
 
+def test_no_app_is_built_with_packed_arithmetic(monkeypatch):
+    """The test and benchmark apps hold kernels too, and so do the sanitizer builds of them."""
+    import __graft_entry__ as entry
+    lines = []
+    monkeypatch.setattr(entry.subprocess, "run", lambda words, **_: lines.append(" ".join(words)))
+    entry.build_apps()
+    for script in ("build_ubsan.sh", "build_tsan.sh"):
+        with open(os.path.join(REPO, "scripts", script)) as f:
+            lines += f.read().replace("\\\n", " ").splitlines()
+    hip = [line for line in lines if line.startswith("/opt/rocm/bin/hipcc")]
+    assert len(hip) == 4
+    for line in hip:
+        assert "-Xclang -target-feature -Xclang -packed-fp32-ops" in line, line
+
+
 @pytest.fixture(scope="module")
 def shipped(tmp_path_factory):
     """The assembly of both units over gp_kernels.hpp, by the Makefile's own commands."""
