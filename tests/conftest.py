@@ -14,6 +14,12 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "slow: full-size (BASELINE) shapes")
 
 
+def pytest_collection_modifyitems(items):
+    # some machines refuse to page-lock memory that exists already, and this test
+    # asks for it: last, so that a run that stops there has run all others
+    items.sort(key=lambda item: item.name == "test_buffers_are_page_locked_on_a_gpu_box")
+
+
 # One summary line per BASELINE config and per hot-path parity family, so the
 # tail of a run's log says which configs ran the HIP path against the oracle.
 # (label, test-file stem, test-function prefixes); first match wins.
