@@ -65,8 +65,10 @@ class _On:
     def __init__(self, device, stream):
         self.guard = [torch.cuda.device(device)]
         if stream is not None:
-            if not hasattr(stream, "cuda_stream"):
-                stream = torch.cuda.ExternalStream(int(stream), device=device)
+            if not hasattr(stream, "cuda_stream"):  # a raw hipStream_t: 0 is the device's null stream
+                handle = int(stream)
+                stream = (torch.cuda.ExternalStream(handle, device=device) if handle
+                          else torch.cuda.default_stream(device))
             if stream.device != device:
                 raise ValueError("stream of another device than the tensors")
             self.guard.append(torch.cuda.stream(stream))
