@@ -133,7 +133,7 @@ class GradPlan:
         return total
 
     def norm(self, stream=None) -> torch.Tensor:
-        """The gradients' norm: one float32 value."""
+        """The gradients' norm: one float32 value (infinity past float32's range)."""
         self._open()
         with _On(self.device, stream):
             return self.sum_squares().sqrt().float()
@@ -213,7 +213,8 @@ def apply_updates_clipped(master: torch.Tensor, updates: Sequence[torch.Tensor],
                           total: torch.Tensor | None = None, skip_nonfinite: bool = False,
                           stream=None) -> torch.Tensor:
     """``out = master + f * u`` for ``u = updates[0] + updates[1] + ...`` (in 32
-    bits, in order) with u's norm bounded; returns the norm, one float32 value.
+    bits, in order) with u's norm bounded; returns the norm, one float32 value
+    (infinity past float32's range; f goes by the 64-bit norm).
     ``out`` defaults to the master.  ``scratch`` (as long as the master) holds u
     between the passes from three updates on; it is allocated when not given.
     ``total``: the sum of squares to go by, over all tables or ranks; u is then

@@ -349,8 +349,11 @@ void launch_sum_square(int nb, float *sum, const Streams &b, size_t n, double *p
 #undef GP_CASE
 }
 
-// From three buckets on their sum is left in `scratch` between the passes
-// (N + 4 streams in all); one or two are read again (2 N + 2).
+// From three buckets on their sum is left in `scratch` between the passes: N + 4
+// streams in all up to kMostStreams buckets.  Each further kMostStreams take a
+// launch of their own, which reads that sum and writes it again: N + 6 from 9 to
+// 16, N + 8 at 17 (61 M floats: 8 buckets 467 us, 9 578, 16 859, 17 979; 64 K
+// floats: 17.6, 20.8, 24.7, 28.1).  One or two are read again (2 N + 2).
 constexpr int kReread = 2;
 
 int launch_squares(float *scratch, const float *const *buckets, int nb, size_t n, double *partial, unsigned *partials,

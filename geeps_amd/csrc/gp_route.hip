@@ -648,6 +648,14 @@ constexpr size_t kMostSortBlocks = 1024;
 //   6000 of 2048 bf16, 4 choices (123 MB)           28.1 us, 27.6
 //   10000 of 4000 bf16, 1 choice (160 MB)           35.3 us, 32.3
 //   8192 of 2048 bf16, 6 choices (235 MB)           47.2 us, 46.0
+// The groups' padding is not counted: it is cleared after the moves, a block its
+// share, by as many blocks as there are tokens, at most two to a CU.  From about
+// 100 tokens that costs nothing (110 of 7168 bf16, 10 choices, 33344 rows, nearly
+// all padding: 103 us, 102; 200 of 2048, 8 choices, 17728 rows: 18.7, 20.4); 17
+// tokens are too few blocks (64 choices of 1024 experts in groups of 64, 65600
+// rows of 4096: 267 us, 105).  The form of up to 1024 choices counts them in every
+// block, those of padding too (128 choices of 512 experts in groups of 64, 8192
+// rows of 7168: 25.9 us, 30.1).
 constexpr size_t kPlaceAndMove = (size_t)96 << 20;
 
 struct SortPlan {
@@ -971,8 +979,14 @@ int gp_route_combine_grad(void *d_rows, size_t d_stride, void *d_weights, const 
   // of 1000 floats, 4 choices: 99 us, 105 with two, 113 with one); two where the
   // row has two steps for them (16384 of 600 bf16, 8 choices: 72 us, 88 with
   // four); one for short rows off a 16-byte boundary, whose lines they would
-  // share (8192 of 1001 bf16, 3 choices: 26 us, 28 with two, 40 with four; not
-  // for few tokens), and for rows of one step.
+  // share, and for rows of one step.  Short rows off the boundary want four waves
+  // while tokens are few, and where that ends lies between 2000 and 4000 tokens by
+  // width and type; 4096 is late for the narrowest.  One wave, two, four:
+  //                              2000 tokens        4000 tokens        8192 tokens
+  //   1001 bf16, 3 choices    14.4 14.7 10.7 us  14.1 14.2 20.3 us  23.6 27.0 36.1 us
+  //   333 floats, 4 choices   14.6 14.6 11.3     14.3 14.4 14.7     20.6 22.2 28.3
+  //   777 floats, 5 choices   14.5 14.5 16.5     26.6 27.2 28.4     52.0 49.2 51.3
+  //   1999 fp16, 4 choices    15.7 15.4 18.4     27.3 28.5 32.8     50.9 51.7 58.9
   const bool aligned = rows_start_at(16, rows_in, row_stride, type);
   const size_t step = kWave * 16 / type_size(type), steps = (width + step - 1) / step;
   const bool one = steps <= 1 || (!aligned && steps <= 4 && tokens >= 4096);

@@ -399,8 +399,8 @@ int gp_route_dispatch(void *out, size_t out_stride, const void *x, size_t x_stri
                       const int32_t *position, const int32_t *order, size_t tokens, size_t k, size_t rows,
                       size_t width, gp_stream s);
 /* gp_route_sort, then gp_route_dispatch of the gp_route_rows() rows: one launch
- * up to 1024 choices; and up to GP_ROUTE_UNCOUNTED of them where tokens
- * and rows are within 96 MiB. */
+ * up to 1024 choices; and up to GP_ROUTE_UNCOUNTED of them where the tokens
+ * and the choices' rows (no padding counted) are within 96 MiB. */
 int gp_route_sort_dispatch(void *out, size_t out_stride, const void *x, size_t x_stride, int type, const void *ids,
                            int id_bits, size_t tokens, size_t k, size_t experts, size_t align, size_t width,
                            int32_t *position, int32_t *order, int32_t *counts, int32_t *offsets, void *workspace,
@@ -408,7 +408,9 @@ int gp_route_sort_dispatch(void *out, size_t out_stride, const void *x, size_t x
 /* y[t] = sum over c of weights[t * k + c] * rows_in[position[t * k + c]],
  * choices in order, those without a row left out (a token with none: zeros).
  * weights: GP_F32 or the rows' type; NULL: 1 each, which is the gradient of
- * gp_route_dispatch.  y must not overlap the rows. */
+ * gp_route_dispatch.  y must not overlap the rows.  (Rows of one stride that
+ * pass between each other, as columns of one buffer, do not overlap, here and in
+ * the other moves; of two strides the whole spans must be apart.) */
 int gp_route_combine(void *y, size_t y_stride, const void *rows_in, size_t row_stride, int type,
                      const int32_t *position, const void *weights, int weight_type, size_t tokens, size_t k,
                      size_t rows, size_t width, gp_stream s);
@@ -430,7 +432,8 @@ int gp_route_combine_grad(void *d_rows, size_t d_stride, void *d_weights, const 
  * (GP_CLIP_PROPAGATE), or drops the update: zeros, an unchanged master
  * (GP_CLIP_SKIP).  `workspace`: GP_CLIP_WORKSPACE_BYTES of device memory, 8-B
  * aligned, any contents, one for each call in flight.  `norm` (device, may be
- * NULL) gets the norm.  Same inputs, same bits.
+ * NULL) gets the norm, rounded to 32 bits: infinity where it passes their range,
+ * though f, and what is skipped, go by the 64-bit value.  Same inputs, same bits.
  * With `sum` (device) given, its sum of squares is used and the values are not
  * squared again: the way to a norm over several lists, tables or ranks, whose
  * gp_*_sum_squares are added up in between.
