@@ -101,7 +101,7 @@ class GradPlan:
         # what the table points at: it must not be given to other tensors, and must be what the tensors still hold
         self._tensors = (*self.grads, *(() if outs is None else self.outs))
         self._storages = [t.untyped_storage() for t in self._tensors]
-        self._facts, self._moved = native.tensor_facts().facts(self._tensors), native.tensor_facts().moved
+        facts = native.tensor_facts()
         n = len(self.grads)
         ptrs, ints, sizes = ctypes.c_void_p * n, ctypes.c_int * n, ctypes.c_size_t * n
         with torch.cuda.device(self.device):
@@ -110,6 +110,8 @@ class GradPlan:
                 ints(*[_TYPES[g.dtype] for g in self.grads]), ptrs(*[o.data_ptr() for o in self.outs]),
                 ints(*[_TYPES[o.dtype] for o in self.outs]), sizes(*[g.numel() for g in self.grads])),
                 "gp_grad_plan_create")
+        # (after data_ptr(), which gives a copy-on-write clone memory of its own)
+        self._facts, self._moved = facts.facts(self._tensors), facts.moved
 
     def _open(self):
         if not self._h:

@@ -112,3 +112,16 @@ def test_a_plan_keeps_the_memory_that_it_points_at(dev):
         torch.cuda.synchronize()
         assert all(bool((t == 3.0).all()) for t in others) and not bool(grad.any())
     plan.close()
+
+
+@pytest.mark.gpu
+def test_a_plan_of_copy_on_write_clones(dev):
+    """Asking for a clone's address gives it memory of its own: that is the plan's, and no move."""
+    base = torch.full((5000,), 2.0, device=dev)
+    grads, outs = [torch._lazy_clone(base)], [torch._lazy_clone(base)]
+    plan = clipping.GradPlan(grads, outs)
+    for _ in range(2):
+        plan.clip(1.0)
+    f = 1.0 / (4.0 * 5000) ** 0.5
+    assert bool((base == 2.0).all()) and bool((grads[0] == 2.0).all())
+    assert bool(((outs[0].double() - 2.0 * f).abs() <= 3 * 2.0 ** -24 * 2.0 * f).all())
